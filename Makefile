@@ -5,7 +5,7 @@ ARCH  ?= gfx950
 HIPFLAGS = -O3 -std=c++17 --offload-arch=$(ARCH) -fPIC -Wall -Wno-unused-result
 
 LIB  = v2e2v_amd/libcista_hip.so
-OBJ  = build/cista_abi.o build/cista_voxel.o build/cista_ssim.o build/cista_v2e.o
+OBJ  = build/cista_abi.o build/cista_voxel.o build/cista_ssim.o build/cista_v2e.o build/cista_optim.o
 
 all: $(LIB)
 
@@ -25,6 +25,11 @@ build/cista_ssim.o: v2e2v_amd/csrc/cista_ssim.hip include/cista_loss.h include/c
 build/cista_v2e.o: v2e2v_amd/csrc/cista_v2e.hip include/cista_v2e.h include/cista_voxel.h include/cista_lstc.h
 	@mkdir -p build
 	$(HIPCC) $(HIPFLAGS) -c -o $@ $<
+
+# packed float32 operations stay off in this file: some forms have given wrong results on gfx950
+build/cista_optim.o: v2e2v_amd/csrc/cista_optim.hip include/cista_optim.h include/cista_lstc.h
+	@mkdir -p build
+	$(HIPCC) $(HIPFLAGS) -Xclang -target-feature -Xclang -packed-fp32-ops -c -o $@ $<
 
 $(LIB): $(OBJ)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -o $@ $(OBJ)

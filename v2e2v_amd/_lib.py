@@ -124,6 +124,13 @@ def _declare(lib):
                                        c_void_p, c_void_p, c_size_t, c_void_p]),
         "cista_ssim_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                         c_void_p, c_void_p, c_size_t, c_void_p]),
+        # include/cista_optim.h (tables as pointers; see optim.py)
+        "cista_optim_workspace_bytes": (c_size_t, [c_int]),
+        "cista_grad_norm": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+        "cista_scale_grads": (c_int, [c_void_p, c_int, ctypes.c_double, c_void_p, c_void_p]),
+        "cista_clip_grads": (c_int, [c_void_p, c_int, c_int, ctypes.c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
+        "cista_adam_step": (c_int, [c_void_p, c_void_p, c_int, c_int, ctypes.c_double, c_void_p, c_void_p, c_size_t,
+                                    c_void_p]),
         # include/cista_v2e.h (config / host-state structs: v2e2v_amd/v2e.py)
         "cista_v2e_state_bytes": (c_size_t, [c_int, c_int, c_int]),
         "cista_v2e_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),

@@ -1,0 +1,551 @@
+// Gradient norm, clipping and the Adam step over many tensors (include/cista_optim.h).
+//
+// All of them stream: 1 to 12 operations per 4 to 28 bytes, so they are bound by HBM for large
+// models and by launches for small ones.  The tensors' table travels in the kernel argument
+// (at most 4 KB), so nothing is uploaded or kept between calls; the work is cut into chunks, and a
+// wave finds a chunk's tensor by one comparison per lane and a ballot.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <vector>
+
+#include "../../include/cista_lstc.h"
+#include "../../include/cista_optim.h"
+
+namespace cista_optim {
+
+constexpr int THREADS = 256;
+constexpr int NORM_TENSORS = 192;        // 20 B each in the kernel argument
+constexpr int NORM_BLOCKS = 2048;        // partial sums of one launch
+constexpr int NORM_UNROLL = 4;           // 16-byte loads in flight per thread
+constexpr int NORM_CHUNK = THREADS * 16 * NORM_UNROLL;                   // bytes
+constexpr int ADAM_TENSORS = 64;         // 52 B each
+constexpr int ADAM_BLOCKS = 2048;
+constexpr int ADAM_CHUNK = THREADS * 4;  // elements
+
+// chunk c belongs to the last tensor whose first chunk is <= c (unused entries: ~0u; an empty
+// tensor's first chunk is the next one's, which is found in its place)
+struct NormTable {
+    void *data[NORM_TENSORS];
+    uint64_t info[NORM_TENSORS];         // numel | type << 56
+    uint32_t first[NORM_TENSORS];
+    uint32_t chunks, pad;
+};
+
+struct AdamTable {
+    void *param[ADAM_TENSORS];
+    const void *grad[ADAM_TENSORS];
+    float *exp_avg[ADAM_TENSORS], *exp_avg_sq[ADAM_TENSORS], *master[ADAM_TENSORS];
+    uint64_t info[ADAM_TENSORS];
+    uint32_t first[ADAM_TENSORS];
+    uint32_t chunks, pad;
+};
+
+struct StepTable {
+    float *step[ADAM_TENSORS];
+};
+
+// what a tensor's update takes from its step count: lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
+struct Rates {
+    float size, inv_root, keep, pad;
+};
+
+__device__ inline float to_f32(float x) { return x; }
+__device__ inline float to_f32(__bf16 x) { return (float)x; }
+__device__ inline float to_f32(_Float16 x) { return (float)x; }
+
+// V elements at p, which is aligned to T only
+template <typename T, int V> struct Pack {
+    T e[V];
+};
+template <typename T, int V> __device__ inline Pack<T, V> load(const T *p) {
+    Pack<T, V> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <typename T, int V> __device__ inline void store(T *p, const Pack<T, V> &r) {
+    __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// the 16-bit value of a float32 result as it is stored: an opaque register keeps the compiler from
+// rounding the last fma to 16 bits at once (v_fma_mixlo_f16), which is another value near a tie
+template <typename T> __device__ inline T rounded(float x) {
+    asm("" : "+v"(x));
+    return (T)x;
+}
+
+template <int N> struct Finder {
+    uint32_t first[(N + 63) / 64];
+    __device__ explicit Finder(const uint32_t *table) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < (N + 63) / 64; ++k) first[k] = table[lane + 64 * k];
+    }
+    __device__ int operator()(uint32_t chunk) const {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < (N + 63) / 64; ++k) n += __popcll(__ballot(first[k] <= chunk));
+        return n - 1;
+    }
+};
+
+// ---------------------------------------------------------------------------------- norm
+// A running value of a norm: a float64 sum, or the largest magnitude as float bits (they order
+// like the magnitudes, and a NaN's lie above infinity's).
+template <int KIND> struct Running {
+    double sum = 0.0;
+    __device__ void add(float x) {
+        if (KIND == CISTA_NORM_2) sum = __builtin_fma((double)x, (double)x, sum);
+        else sum += (double)__builtin_fabsf(x);
+    }
+    __device__ void join(const Running &o) { sum += o.sum; }
+    __device__ double bits() const { return sum; }
+    __device__ static Running of(double b) {
+        Running r;
+        r.sum = b;
+        return r;
+    }
+    __device__ Running from(int lane) const { return of(__shfl_xor(sum, lane)); }
+    __device__ float value() const { return (float)(KIND == CISTA_NORM_2 ? __builtin_sqrt(sum) : sum); }
+};
+template <> struct Running<CISTA_NORM_MAX> {
+    uint32_t most = 0;
+    __device__ void add(float x) { most = max(most, __float_as_uint(x) & 0x7fffffffu); }
+    __device__ void join(const Running &o) { most = max(most, o.most); }
+    __device__ double bits() const { return __longlong_as_double((long long)most); }
+    __device__ static Running of(double b) {
+        Running r;
+        r.most = (uint32_t)__double_as_longlong(b);
+        return r;
+    }
+    __device__ Running from(int lane) const {
+        Running r;
+        r.most = __shfl_xor(most, lane);
+        return r;
+    }
+    __device__ float value() const { return __uint_as_float(most); }
+};
+
+// the block's value, in every thread
+template <int KIND> __device__ Running<KIND> block_join(Running<KIND> r) {
+    __shared__ double part[THREADS / 64];
+#pragma unroll
+    for (int l = 32; l; l >>= 1) r.join(r.from(l));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = r.bits();
+    __syncthreads();
+    r = Running<KIND>::of(part[0]);
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) r.join(Running<KIND>::of(part[w]));
+    return r;
+}
+
+template <int KIND, typename T>
+__device__ void norm_chunk(Running<KIND> (&acc)[NORM_UNROLL], const T *g, uint64_t left) {
+    constexpr int V = 16 / sizeof(T);
+    const uint32_t at = threadIdx.x * V;
+    if (left >= (uint64_t)NORM_UNROLL * THREADS * V) {
+        Pack<T, V> x[NORM_UNROLL];
+#pragma unroll
+        for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<T, V>(g + at + u * THREADS * V);
+#pragma unroll
+        for (int u = 0; u < NORM_UNROLL; ++u)
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[u].add(to_f32(x[u].e[e]));
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < NORM_UNROLL; ++u) {
+        const uint32_t i = at + u * THREADS * V;
+        if (i + V <= left) {
+            const Pack<T, V> x = load<T, V>(g + i);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[u].add(to_f32(x.e[e]));
+        } else {
+            for (uint32_t e = i; e < left; ++e) acc[u].add(to_f32(g[e]));
+        }
+    }
+}
+
+template <int KIND> __global__ __launch_bounds__(THREADS) void norm_partials_kernel(NormTable t, double *partials) {
+    const Finder<NORM_TENSORS> find(t.first);
+    Running<KIND> acc[NORM_UNROLL];
+    for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+        const int i = find(c);
+        const uint64_t info = t.info[i], off = (uint64_t)(c - t.first[i]) * NORM_CHUNK;
+        const char *g = (const char *)t.data[i] + off;
+        const uint64_t numel = info & ((1ull << 56) - 1);
+        switch (info >> 56) {
+        case CISTA_F32: norm_chunk<KIND>(acc, (const float *)g, numel - off / 4); break;
+        case CISTA_BF16: norm_chunk<KIND>(acc, (const __bf16 *)g, numel - off / 2); break;
+        default: norm_chunk<KIND>(acc, (const _Float16 *)g, numel - off / 2); break;
+        }
+    }
+#pragma unroll
+    for (int u = 1; u < NORM_UNROLL; ++u) acc[0].join(acc[u]);
+    const Running<KIND> r = block_join(acc[0]);
+    if (threadIdx.x == 0) partials[blockIdx.x] = r.bits();
+}
+
+template <int KIND> __device__ float norm_of(const double *partials, int n) {
+    Running<KIND> r;
+    for (int i = threadIdx.x; i < n; i += THREADS) r.join(Running<KIND>::of(partials[i]));
+    return block_join(r).value();
+}
+
+template <int KIND> __global__ __launch_bounds__(THREADS) void norm_join_kernel(const double *partials, int n, float *norm) {
+    const float v = norm_of<KIND>(partials, n);
+    if (threadIdx.x == 0) *norm = v;
+}
+
+// ---------------------------------------------------------------------------------- scale
+__device__ inline float clip_scale(float norm, double max_norm) {
+    if (max_norm == __builtin_inf()) return 1.0f;
+    const double c = max_norm / ((double)norm + 1e-6);
+    return c >= 1.0 ? 1.0f : (float)c;       // a NaN stays one
+}
+
+template <typename T> __device__ void scale_chunk(T *g, uint64_t left, float c) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < NORM_UNROLL; ++u) {
+        const uint32_t i = (threadIdx.x + u * THREADS) * V;
+        if (i + V <= left) {
+            Pack<T, V> x = load<T, V>(g + i);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x.e[e] = (T)(to_f32(x.e[e]) * c);
+            store<T, V>(g + i, x);
+        } else {
+            for (uint32_t e = i; e < left; ++e) g[e] = (T)(to_f32(g[e]) * c);
+        }
+    }
+}
+
+// one rounding to the gradient's type, of a float32 product
+__global__ __launch_bounds__(THREADS) void scale_kernel(NormTable t, double max_norm, const float *norm) {
+    const float c = clip_scale(*norm, max_norm);
+    if (c == 1.0f) return;                   // x * 1 is x for every x: nothing to read or write
+    const Finder<NORM_TENSORS> find(t.first);
+    for (uint32_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
+        const int i = find(k);
+        const uint64_t info = t.info[i], off = (uint64_t)(k - t.first[i]) * NORM_CHUNK;
+        char *g = (char *)t.data[i] + off;
+        const uint64_t numel = info & ((1ull << 56) - 1);
+        switch (info >> 56) {
+        case CISTA_F32: scale_chunk((float *)g, numel - off / 4, c); break;
+        case CISTA_BF16: scale_chunk((__bf16 *)g, numel - off / 2, c); break;
+        default: scale_chunk((_Float16 *)g, numel - off / 2, c); break;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------- Adam
+struct AdamArgs {
+    double lr, log_beta1, log_beta2, weight_decay, max_norm;
+    const float *lr_device;
+    float rate1, rate2, eps;                 // 1 - b1, 1 - b2
+    float decay;                             // in the gradient; 0 where it is decoupled
+    int decoupled, maximize;
+};
+
+static_assert(sizeof(NormTable) + 32 <= 4096 && sizeof(AdamTable) + sizeof(AdamArgs) + 32 <= 4096, "kernel arguments");
+
+__global__ void adam_advance_kernel(StepTable s, int n, AdamArgs a, Rates *rates) {
+    const int i = threadIdx.x;
+    if (i >= n) return;
+    const float t = *s.step[i] + 1.0f;
+    *s.step[i] = t;
+    const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
+    // 1 - b^t without the cancellation of small t; log(0) = -inf gives 1
+    Rates r;
+    r.size = (float)(lr / -expm1((double)t * a.log_beta1));
+    r.inv_root = (float)(1.0 / sqrt(-expm1((double)t * a.log_beta2)));
+    r.keep = a.decoupled ? (float)(1.0 - lr * a.weight_decay) : 1.0f;
+    r.pad = 0.0f;
+    rates[i] = r;
+}
+
+__device__ inline void adam_element(float &p, float g, float &m, float &v, const AdamArgs &a, const Rates &r, float c) {
+    g *= c;
+    g = a.maximize ? -g : g;
+    if (a.decay != 0.0f) g = fmaf(a.decay, p, g);
+    p *= r.keep;
+    m = fmaf(a.rate1, g - m, m);
+    // b2 v as v - (1 - b2) v: float32 holds 1 - b2 to 2^-24 of itself, b2 only to 2^-24 of 1, which
+    // would move the average of a long run by 2^-24 / (1 - b2)
+    const float kept = v < __builtin_inff() ? fmaf(-a.rate2, v, v) : v;
+    v = fmaf(a.rate2 * g, g, kept);
+    p = fmaf(-r.size, m / fmaf(sqrtf(v), r.inv_root, a.eps), p);
+}
+
+template <typename T>
+__device__ void adam_chunk(T *p, const T *g, float *m, float *v, float *w, uint64_t left, const AdamArgs &a,
+                           const Rates &r, float c) {
+    const uint32_t i = threadIdx.x * 4;
+    if (i + 4 <= left) {
+        const Pack<T, 4> gx = load<T, 4>(g + i);
+        Pack<float, 4> wx = load<float, 4>(w + i), mx = load<float, 4>(m + i), vx = load<float, 4>(v + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) adam_element(wx.e[e], to_f32(gx.e[e]), mx.e[e], vx.e[e], a, r, c);
+        store(m + i, mx);
+        store(v + i, vx);
+        store(w + i, wx);
+        if (sizeof(T) != 4) {
+            Pack<T, 4> px;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) px.e[e] = rounded<T>(wx.e[e]);
+            store(p + i, px);
+        }
+    } else {
+        for (uint32_t e = i; e < left; ++e) {
+            adam_element(w[e], to_f32(g[e]), m[e], v[e], a, r, c);
+            if (sizeof(T) != 4) p[e] = rounded<T>(w[e]);
+        }
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void adam_kernel(AdamTable t, AdamArgs a, const Rates *rates, const float *norm) {
+    const Finder<ADAM_TENSORS> find(t.first);
+    const float c = norm ? clip_scale(*norm, a.max_norm) : 1.0f;
+    for (uint32_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
+        const int i = find(k);
+        const uint64_t info = t.info[i], off = (uint64_t)(k - t.first[i]) * ADAM_CHUNK;
+        const uint64_t left = (info & ((1ull << 56) - 1)) - off;
+        const Rates r = rates[i];
+        float *m = t.exp_avg[i] + off, *v = t.exp_avg_sq[i] + off;
+        switch (info >> 56) {
+        case CISTA_F32:
+            adam_chunk((float *)t.param[i] + off, (const float *)t.grad[i] + off, m, v, (float *)t.param[i] + off, left,
+                       a, r, c);
+            break;
+        case CISTA_BF16:
+            adam_chunk((__bf16 *)t.param[i] + off, (const __bf16 *)t.grad[i] + off, m, v, t.master[i] + off, left, a, r,
+                       c);
+            break;
+        default:
+            adam_chunk((_Float16 *)t.param[i] + off, (const _Float16 *)t.grad[i] + off, m, v, t.master[i] + off, left,
+                       a, r, c);
+            break;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------- host
+inline int size_of(long long type) { return type == CISTA_F32 ? 4 : 2; }
+inline int hip_ok() { return hipGetLastError() == hipSuccess ? CISTA_OK : CISTA_ERR_HIP; }
+inline int launches(int n, int per) { return n <= 0 ? 1 : (n + per - 1) / per; }
+
+// 2^40 elements in all keep the chunk counts below 2^31
+bool bad_tensor(const void *data, long long numel, long long type) {
+    if (numel < 0 || type < CISTA_F32 || type > CISTA_F16) return true;
+    return numel > 0 && (!data || (uintptr_t)data % size_of(type));
+}
+
+struct Range {
+    uintptr_t begin, end;
+};
+
+// Do the n ranges of get(i) overlap?  Tensors that lie in their list's order, as views of one
+// buffer do, need no sorting.
+template <typename Get> int overlap(int n, Get get) {
+    uintptr_t end = 0;
+    int i = 0;
+    for (; i < n; ++i) {
+        const Range r = get(i);
+        if (r.begin == r.end) continue;
+        if (r.begin < end) break;
+        end = r.end;
+    }
+    if (i == n) return CISTA_OK;
+    try {
+        std::vector<Range> all;
+        all.reserve(n);
+        for (i = 0; i < n; ++i)
+            if (get(i).begin != get(i).end) all.push_back(get(i));
+        std::sort(all.begin(), all.end(), [](const Range &x, const Range &y) { return x.begin < y.begin; });
+        for (size_t k = 1; k < all.size(); ++k)
+            if (all[k].begin < all[k - 1].end) return CISTA_ERR_ALIAS;
+    } catch (...) {
+        return CISTA_ERR_HIP;
+    }
+    return CISTA_OK;
+}
+
+Range range_of(const void *data, long long numel, long long type) {
+    return {(uintptr_t)data, (uintptr_t)data + (uintptr_t)numel * size_of(type)};
+}
+
+int check(const cista_tensor *t, int n, bool written) {
+    if (n < 0 || (n && !t)) return CISTA_ERR_INVALID;
+    long long total = 0;
+    for (int i = 0; i < n; ++i) {
+        if (bad_tensor(t[i].data, t[i].numel, t[i].type)) return CISTA_ERR_INVALID;
+        if (t[i].numel >> 40 || (total += t[i].numel) >> 40) return CISTA_ERR_UNSUPPORTED;
+    }
+    if (!written) return CISTA_OK;
+    return overlap(n, [&](int i) { return range_of(t[i].data, t[i].numel, t[i].type); });
+}
+
+// Fills tables of NORM_TENSORS tensors and calls f(table, blocks) for each.
+template <typename Get, typename F> void each_table(int n, Get get, F f) {
+    for (int i = 0; i < n;) {
+        NormTable t;
+        int k = 0;
+        uint64_t chunks = 0;
+        for (; i < n && k < NORM_TENSORS; ++i) {
+            const cista_tensor x = get(i);
+            if (!x.numel) continue;
+            t.data[k] = x.data;
+            t.info[k] = (uint64_t)x.numel | (uint64_t)x.type << 56;
+            t.first[k++] = (uint32_t)chunks;
+            chunks += ((uint64_t)x.numel * size_of(x.type) + NORM_CHUNK - 1) / NORM_CHUNK;
+        }
+        if (!k) break;
+        for (int j = k; j < NORM_TENSORS; ++j) t.data[j] = nullptr, t.info[j] = 0, t.first[j] = ~0u;
+        t.chunks = (uint32_t)chunks;
+        t.pad = 0;
+        f(t, (int)std::min<uint64_t>(chunks, NORM_BLOCKS));
+    }
+}
+
+template <int KIND, typename Get> int norm_launch(int n, Get get, float *norm, double *partials, hipStream_t s) {
+    int used = 0;
+    each_table(n, get, [&](const NormTable &t, int blocks) {
+        norm_partials_kernel<KIND><<<blocks, THREADS, 0, s>>>(t, partials + used);
+        used += blocks;
+    });
+    norm_join_kernel<KIND><<<1, THREADS, 0, s>>>(partials, used, norm);
+    return hip_ok();
+}
+
+template <typename Get> int norm_any(int kind, int n, Get get, float *norm, double *partials, hipStream_t s) {
+    switch (kind) {
+    case CISTA_NORM_1: return norm_launch<CISTA_NORM_1>(n, get, norm, partials, s);
+    case CISTA_NORM_2: return norm_launch<CISTA_NORM_2>(n, get, norm, partials, s);
+    case CISTA_NORM_MAX: return norm_launch<CISTA_NORM_MAX>(n, get, norm, partials, s);
+    }
+    return CISTA_ERR_INVALID;
+}
+
+size_t partial_bytes(int n) { return (size_t)launches(n, NORM_TENSORS) * NORM_BLOCKS * sizeof(double); }
+
+}  // namespace cista_optim
+
+using namespace cista_optim;
+
+extern "C" {
+
+size_t cista_optim_workspace_bytes(int n) {
+    return n < 0 ? 0 : partial_bytes(n) + (size_t)std::max(n, 1) * sizeof(Rates);
+}
+
+int cista_grad_norm(const cista_tensor *grads, int n, int norm_kind, float *norm, void *workspace,
+                    size_t workspace_bytes, void *stream) {
+    const int st = check(grads, n, false);
+    if (st != CISTA_OK) return st;
+    if (!norm || !workspace) return CISTA_ERR_INVALID;
+    if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
+    return norm_any(norm_kind, n, [&](int i) { return grads[i]; }, norm, (double *)workspace, (hipStream_t)stream);
+}
+
+int cista_scale_grads(const cista_tensor *grads, int n, double max_norm, const float *norm, void *stream) {
+    const int st = check(grads, n, true);
+    if (st != CISTA_OK) return st;
+    if (!norm || !(max_norm >= 0.0)) return CISTA_ERR_INVALID;
+    each_table(n, [&](int i) { return grads[i]; }, [&](const NormTable &t, int blocks) {
+        scale_kernel<<<blocks, THREADS, 0, (hipStream_t)stream>>>(t, max_norm, norm);
+    });
+    return hip_ok();
+}
+
+int cista_clip_grads(const cista_tensor *grads, int n, int norm_kind, double max_norm, float *norm, void *workspace,
+                     size_t workspace_bytes, void *stream) {
+    if (!(max_norm >= 0.0)) return CISTA_ERR_INVALID;
+    int st = check(grads, n, true);
+    if (st == CISTA_OK) st = cista_grad_norm(grads, n, norm_kind, norm, workspace, workspace_bytes, stream);
+    return st != CISTA_OK ? st : cista_scale_grads(grads, n, max_norm, norm, stream);
+}
+
+int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *groups, int n_groups, int norm_kind,
+                    double max_norm, float *norm, void *workspace, size_t workspace_bytes, void *stream) {
+    if (n_groups < 0 || (n_groups && !groups) || norm_kind < 0 || norm_kind > CISTA_NORM_MAX) return CISTA_ERR_INVALID;
+    if (norm_kind && (!norm || !(max_norm >= 0.0))) return CISTA_ERR_INVALID;
+    int n = 0;
+    for (int k = 0; k < n_groups; ++k) {
+        const cista_adam_group &q = groups[k];
+        if (q.n < 0 || !(q.beta1 >= 0.0 && q.beta1 < 1.0 && q.beta2 >= 0.0 && q.beta2 < 1.0)) return CISTA_ERR_INVALID;
+        n += q.n;
+    }
+    if (n && !table) return CISTA_ERR_INVALID;
+    long long total = 0;
+    for (int i = 0; i < n; ++i) {
+        const cista_adam_tensor &x = table[i];
+        if (bad_tensor(x.param, x.numel, x.type) || bad_tensor(x.grad, x.numel, x.type) || !x.step ||
+            bad_tensor(x.exp_avg, x.numel, CISTA_F32) || bad_tensor(x.exp_avg_sq, x.numel, CISTA_F32) ||
+            (x.type != CISTA_F32 && bad_tensor(x.master, x.numel, CISTA_F32)))
+            return CISTA_ERR_INVALID;
+        if (x.numel >> 40 || (total += x.numel) >> 40) return CISTA_ERR_UNSUPPORTED;
+    }
+    const int apart = overlap(n, [&](int i) { return range_of(table[i].param, table[i].numel, table[i].type); });
+    if (apart != CISTA_OK) return apart;
+    if (!workspace) return CISTA_ERR_INVALID;
+    if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
+    if (norm_kind) {
+        const int st = norm_any(norm_kind, n, [&](int i) {
+            return cista_tensor{(void *)table[i].grad, table[i].numel, table[i].type};
+        }, norm, (double *)workspace, s);
+        if (st != CISTA_OK) return st;
+    }
+    Rates *rates = (Rates *)((char *)workspace + partial_bytes(n));
+    const cista_adam_tensor *x = table;
+    for (int k = 0; k < n_groups; ++k) {
+        const cista_adam_group &q = groups[k];
+        AdamArgs a;
+        a.lr = q.lr;
+        a.log_beta1 = std::log(q.beta1);
+        a.log_beta2 = std::log(q.beta2);
+        a.weight_decay = q.weight_decay;
+        a.max_norm = max_norm;
+        a.lr_device = q.lr_device;
+        a.rate1 = (float)(1.0 - q.beta1);
+        a.rate2 = (float)(1.0 - q.beta2);
+        a.eps = (float)q.eps;
+        a.decay = q.decoupled ? 0.0f : (float)q.weight_decay;
+        a.decoupled = q.decoupled;
+        a.maximize = q.maximize;
+        for (int i = 0; i < q.n; i += ADAM_TENSORS) {
+            AdamTable t;
+            StepTable steps;
+            const int now = std::min(ADAM_TENSORS, q.n - i);
+            uint64_t chunks = 0;
+            int used = 0;
+            for (int j = 0; j < ADAM_TENSORS; ++j) {
+                t.param[j] = nullptr, t.grad[j] = nullptr, t.master[j] = nullptr;
+                t.exp_avg[j] = t.exp_avg_sq[j] = nullptr;
+                t.info[j] = 0, t.first[j] = ~0u;
+                steps.step[j] = j < now ? x[j].step : nullptr;
+            }
+            for (int j = 0; j < now; ++j) {
+                t.param[j] = x[j].param, t.grad[j] = x[j].grad, t.master[j] = x[j].master;
+                t.exp_avg[j] = x[j].exp_avg, t.exp_avg_sq[j] = x[j].exp_avg_sq;
+                t.info[j] = (uint64_t)x[j].numel | (uint64_t)x[j].type << 56;
+                t.first[j] = (uint32_t)chunks;
+                chunks += ((uint64_t)x[j].numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
+                used = j + 1;
+            }
+            t.chunks = (uint32_t)chunks;
+            t.pad = 0;
+            adam_advance_kernel<<<1, ADAM_TENSORS, 0, s>>>(steps, used, a, rates);
+            if (chunks)
+                adam_kernel<<<(int)std::min<uint64_t>(chunks, ADAM_BLOCKS), THREADS, 0, s>>>(t, a, rates,
+                                                                                            norm_kind ? norm : nullptr);
+            x += now;
+            rates += now;
+        }
+    }
+    return hip_ok();
+}
+
+}  // extern "C"
