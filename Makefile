@@ -7,7 +7,13 @@ HIPFLAGS = -O3 -std=c++17 --offload-arch=$(ARCH) -fPIC -Wall -Wno-unused-result
 LIB  = v2e2v_amd/libcista_hip.so
 OBJ  = build/cista_abi.o build/cista_voxel.o build/cista_ssim.o build/cista_v2e.o build/cista_optim.o
 
-all: $(LIB)
+# host library between Python's lists of tensors and the C ABI (links the installed torch)
+TLIB  = v2e2v_amd/libcista_torch.so
+PY    ?= python3
+TORCH = $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(u.find_spec('torch').origin))")
+PYINC = $(shell $(PY) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+
+all: $(LIB) $(TLIB)
 
 build/cista_abi.o: v2e2v_amd/csrc/cista_abi.hip v2e2v_amd/csrc/cista_kernels.hpp \
                    v2e2v_amd/csrc/cista_backward.hpp include/cista_lstc.h
@@ -34,7 +40,12 @@ build/cista_optim.o: v2e2v_amd/csrc/cista_optim.hip include/cista_optim.h includ
 $(LIB): $(OBJ)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -o $@ $(OBJ)
 
+$(TLIB): v2e2v_amd/csrc/cista_torch.cpp include/cista_optim.h include/cista_lstc.h
+	$(CXX) -O2 -std=c++17 -fPIC -Wall -shared -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -I$(PYINC) -isystem $(TORCH)/include \
+	    -isystem $(TORCH)/include/torch/csrc/api/include -isystem /opt/rocm/include -o $@ $< \
+	    -L$(TORCH)/lib -ltorch_python -ltorch_cpu -lc10 -lc10_hip
+
 clean:
-	rm -rf build $(LIB)
+	rm -rf build $(LIB) $(TLIB)
 
 .PHONY: all clean

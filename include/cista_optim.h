@@ -75,7 +75,8 @@ typedef struct {
 /* One step over all groups; the table holds the groups' tensors one group after the other.
  * norm_kind 0: no clipping (max_norm and norm are not used); else every gradient is scaled by c
  * of the norm over all groups, which goes to *norm; the gradients in memory stay as they are.
- * The parameters are disjoint (checked: CISTA_ERR_ALIAS). */
+ * The parameters are disjoint, and so are the m, the v, the master copies and the steps (checked:
+ * CISTA_ERR_ALIAS). */
 int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *groups, int n_groups, int norm_kind,
                     double max_norm, float *norm, void *workspace, size_t workspace_bytes, void *stream);
 

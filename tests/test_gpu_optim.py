@@ -27,6 +27,14 @@ DEV = "cuda"
 ODD = [1, 2, 3, 5, 7, 8, 9, 0, 63, 65, 255, 257, 1023, 1024, 1025, 4095, 4096, 4097, 8191, 8192, 8193, 0, 30011]
 
 
+@pytest.fixture(autouse=True, params=["short", "python"])
+def way(request, monkeypatch):
+    """Each test through csrc/cista_torch.cpp where it takes the call, and through Python alone."""
+    if request.param == "python":
+        monkeypatch.setattr(optim, "_short", lambda *args: NotImplemented)
+    return request.param
+
+
 def gen(seed):
     return torch.Generator(device=DEV).manual_seed(seed)
 
@@ -450,6 +458,31 @@ def test_folded_clipping_is_clipping_and_then_the_step():
             runs.append([p.detach().clone() for p in ps] + [opt.grad_norm if folded else norm])
     for a, b in zip(runs[:4], runs[4:]):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_the_short_way_is_taken(way, monkeypatch):
+    """What a training step does goes through csrc/cista_torch.cpp; what that leaves to Python works too."""
+    if way == "python":
+        pytest.skip("only the short way")
+    ps, _ = adam_case([5, 3000], torch.bfloat16, 12, 0)
+    opt = optim.Adam([dict(params=ps, lr=torch.tensor(0.1, device=DEV))], max_norm=1.0)
+    opt.step()                                            # makes the state, in Python
+    taken = []
+    real = optim._short
+    monkeypatch.setattr(optim, "_short", lambda *a: taken.append(real(*a)) or taken[-1])
+    optim.grad_norm([p.grad for p in ps])
+    optim.grad_norm(tuple(p.grad for p in ps))
+    optim.clip_grad_norm_(iter(ps), 1.0)
+    opt.step()
+    assert len(taken) == 4 and all(isinstance(t, torch.Tensor) for t in taken)
+    ps[0].grad = ps[0].grad.new_ones(10)[::2]
+    optim.clip_grad_norm_(ps, 1.0)
+    assert taken[-1] is NotImplemented
+    ps[0].grad = torch.ones_like(ps[0])
+    plain = optim.Adam(ps)
+    plain.step()
+    plain.step()
+    assert taken[-1] is None
 
 
 def test_equal_inputs_give_equal_bits():

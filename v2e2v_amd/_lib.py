@@ -167,6 +167,29 @@ def lib():
     return _lib
 
 
+_torch_lib = None
+TORCH_LIB_PATH = os.path.join(_HERE, "libcista_torch.so")
+
+
+def torch_lib():
+    """Load (once) the host library that reads tables out of lists of tensors (csrc/cista_torch.cpp).
+    It takes its calls of include/ from the library that lib() has loaded, and Python objects as
+    they are (PyDLL: the GIL stays held)."""
+    global _torch_lib
+    if _torch_lib is None:
+        lib()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise CistaError(f"libcista_torch.so not found at {TORCH_LIB_PATH}; build it first (`make`)")
+        t = ctypes.PyDLL(TORCH_LIB_PATH)
+        obj, dbl = ctypes.py_object, ctypes.c_double
+        for name, args in (("cista_torch_grad_norm", [obj, c_int]), ("cista_torch_clip_grads", [obj, c_int, dbl]),
+                           ("cista_torch_adam_step", [obj, obj, c_int, dbl])):
+            fn = getattr(t, name)
+            fn.restype, fn.argtypes = obj, args
+        _torch_lib = t
+    return _torch_lib
+
+
 def header_functions(path: str | None = None):
     """Names of every function declared in include/*.h (or in one header `path`)."""
     paths = [path] if path else sorted(

@@ -487,7 +487,16 @@ int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *grou
             return CISTA_ERR_INVALID;
         if (x.numel >> 40 || (total += x.numel) >> 40) return CISTA_ERR_UNSUPPORTED;
     }
-    const int apart = overlap(n, [&](int i) { return range_of(table[i].param, table[i].numel, table[i].type); });
+    int apart = overlap(n, [&](int i) { return range_of(table[i].param, table[i].numel, table[i].type); });
+    for (auto which : {&cista_adam_tensor::exp_avg, &cista_adam_tensor::exp_avg_sq, &cista_adam_tensor::master,
+                       &cista_adam_tensor::step}) {
+        if (apart != CISTA_OK) return apart;
+        apart = overlap(n, [&](int i) {
+            const cista_adam_tensor &x = table[i];
+            const bool none = which == &cista_adam_tensor::master && x.type == CISTA_F32;
+            return range_of(x.*which, which == &cista_adam_tensor::step ? 1 : none ? 0 : x.numel, CISTA_F32);
+        });
+    }
     if (apart != CISTA_OK) return apart;
     if (!workspace) return CISTA_ERR_INVALID;
     if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;

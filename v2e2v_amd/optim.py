@@ -68,11 +68,6 @@ def _check_tensor(t, what):
         raise _lib.CistaError(f"{what} has type {t.dtype}: float32, bfloat16 and float16 are supported")
 
 
-def _dense(t) -> bool:
-    """Whether the elements fill one run of memory, in whatever order of the dimensions."""
-    return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
-
-
 def _same_device(tensors, what):
     dev = tensors[0].device
     for t in tensors:
@@ -105,7 +100,20 @@ def _workspace(n, device):
 
 
 def _as_list(tensors):
-    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    return tensors if type(tensors) is list else [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+
+
+def _short(name, *args):
+    """A call of csrc/cista_torch.cpp: its result, or NotImplemented where it leaves the call to Python."""
+    got = getattr(_lib.torch_lib(), name)(*args)
+    if type(got) is int:
+        _lib.check(got, name.replace("_torch", ""))
+    return got
+
+
+def _dense(t) -> bool:
+    """Whether the elements fill one run of memory, in whatever order of the dimensions."""
+    return (t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)) and not t.is_neg()
 
 
 def _grads(parameters):
@@ -126,11 +134,16 @@ def grad_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
     tensors = _as_list(tensors)
     if not tensors:
         return torch.tensor(0.0)
+    norm = _short("cista_torch_grad_norm", tensors, kind)
+    if norm is not NotImplemented:
+        if error_if_nonfinite:
+            _raise_if_nonfinite(norm, norm_type)
+        return norm
     for t in tensors:
         _check_tensor(t, "tensor")
     dev = _same_device(tensors, "tensors")
     with _on(dev), torch.no_grad():
-        tensors = [t if _dense(t) else t.contiguous() for t in tensors]
+        tensors = [t if _dense(t) else t.resolve_neg().contiguous() for t in tensors]
         norm = torch.empty((), dtype=torch.float32, device=dev)
         ws = _workspace(len(tensors), dev)
         _lib.check(_lib.lib().cista_grad_norm(_table(tensors), len(tensors), kind, norm.data_ptr(), ws.data_ptr(),
@@ -143,7 +156,7 @@ def grad_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
 def _written(grads, call):
     """Runs `call` on dense stand-ins of the gradients, and writes those that are copies back."""
     torch.autograd.graph.increment_version(grads)        # raises for what may not be written
-    dense = [g if _dense(g) else g.contiguous() for g in grads]
+    dense = [g if _dense(g) else g.resolve_neg().contiguous() for g in grads]
     call(dense)
     for g, d in zip(grads, dense):
         if d is not g:
@@ -181,6 +194,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     error_if_nonfinite asks for a RuntimeError before anything is written (which waits for the GPU)."""
     max_norm, kind = _max_norm(max_norm), _norm_kind(norm_type)
     parameters = _as_list(parameters)
+    if not error_if_nonfinite:
+        norm = _short("cista_torch_clip_grads", parameters, kind, max_norm)
+        if norm is not NotImplemented:
+            return norm
     grads = _grads(parameters)
     if not grads:
         return torch.tensor(0.0)
@@ -298,6 +315,11 @@ class Adam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        kind = 0 if self.max_norm is None else _norm_kind(self.norm_type)
+        norm = _short("cista_torch_adam_step", self.param_groups, self.state, kind, self.max_norm or 0.0)
+        if norm is not NotImplemented:
+            self.grad_norm = norm
+            return loss
         rows, groups, keep, changed = [], [], [], []
         for g in self.param_groups:
             params = [p for p in g["params"] if p.grad is not None]
@@ -331,7 +353,6 @@ class Adam(torch.optim.Optimizer):
         if not rows:
             return loss
         dev = _same_device(changed, "parameters")
-        kind = _norm_kind(self.norm_type) if self.max_norm is not None else 0
         torch.autograd.graph.increment_version(changed)      # the network repacks changed weights
         with _on(dev):
             norm = torch.empty((), dtype=torch.float32, device=dev) if kind else None
