@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/cista_lstc.h"
@@ -22,15 +23,16 @@ constexpr int NORM_BLOCKS = 2048;        // partial sums of one launch
 constexpr int NORM_UNROLL = 4;           // 16-byte loads in flight per thread
 constexpr int NORM_CHUNK = THREADS * 16 * NORM_UNROLL;                   // bytes
 constexpr int ADAM_TENSORS = 64;         // 52 B each
+constexpr int STEP_TENSORS = 448;        // 8 B each
 constexpr int ADAM_BLOCKS = 2048;
 constexpr int ADAM_CHUNK = THREADS * 4;  // elements
 
 // chunk c belongs to the last tensor whose first chunk is <= c (unused entries: ~0u; an empty
 // tensor's first chunk is the next one's, which is found in its place)
-struct NormTable {
-    void *data[NORM_TENSORS];
-    uint64_t info[NORM_TENSORS];         // numel | type << 56
-    uint32_t first[NORM_TENSORS];
+template <int N> struct NormTable {
+    void *data[N];
+    uint64_t info[N];                    // numel | type << 56
+    uint32_t first[N];
     uint32_t chunks, pad;
 };
 
@@ -43,13 +45,21 @@ struct AdamTable {
     uint32_t chunks, pad;
 };
 
-struct StepTable {
-    float *step[ADAM_TENSORS];
+template <int N> struct StepTable {
+    float *step[N];
 };
 
 // what a tensor's update takes from its step count: lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
 struct Rates {
     float size, inv_root, keep, pad;
+};
+
+struct AdamArgs {
+    double lr, log_beta1, log_beta2, weight_decay, max_norm;
+    const float *lr_device;
+    float rate1, rate2, eps;                 // 1 - b1, 1 - b2
+    float decay;                             // in the gradient; 0 where it is decoupled
+    int decoupled, maximize;
 };
 
 __device__ inline float to_f32(float x) { return x; }
@@ -90,6 +100,25 @@ template <int N> struct Finder {
         return n - 1;
     }
 };
+
+// t <- t + 1, and what the update takes from it
+__device__ inline void advance(float *step, const AdamArgs &a, Rates *rates) {
+    const float t = *step + 1.0f;
+    *step = t;
+    const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
+    // 1 - b^t without the cancellation of small t; log(0) = -inf gives 1
+    Rates r;
+    r.size = (float)(lr / -expm1((double)t * a.log_beta1));
+    r.inv_root = (float)(1.0 / sqrt(-expm1((double)t * a.log_beta2)));
+    r.keep = a.decoupled ? (float)(1.0 - lr * a.weight_decay) : 1.0f;
+    r.pad = 0.0f;
+    *rates = r;
+}
+
+__global__ void adam_advance_kernel(StepTable<STEP_TENSORS> s, int n, AdamArgs a, Rates *rates) {
+    const int i = threadIdx.x;
+    if (i < n) advance(s.step[i], a, rates + i);
+}
 
 // ---------------------------------------------------------------------------------- norm
 // A running value of a norm: a float64 sum, or the largest magnitude as float bits (they order
@@ -168,10 +197,10 @@ __device__ void norm_chunk(Running<KIND> (&acc)[NORM_UNROLL], const T *g, uint64
     }
 }
 
-template <int KIND> __global__ __launch_bounds__(THREADS) void norm_partials_kernel(NormTable t, double *partials) {
-    const Finder<NORM_TENSORS> find(t.first);
+template <int KIND, int N> __device__ void norm_partials(const NormTable<N> &t, double *partials, uint32_t blocks) {
+    const Finder<N> find(t.first);
     Running<KIND> acc[NORM_UNROLL];
-    for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    for (uint32_t c = blockIdx.x; c < t.chunks; c += blocks) {
         const int i = find(c);
         const uint64_t info = t.info[i], off = (uint64_t)(c - t.first[i]) * NORM_CHUNK;
         const char *g = (const char *)t.data[i] + off;
@@ -188,10 +217,55 @@ template <int KIND> __global__ __launch_bounds__(THREADS) void norm_partials_ker
     if (threadIdx.x == 0) partials[blockIdx.x] = r.bits();
 }
 
+template <int KIND>
+__global__ __launch_bounds__(THREADS) void norm_partials_kernel(NormTable<NORM_TENSORS> t, double *partials) {
+    norm_partials<KIND>(t, partials, gridDim.x);
+}
+
+// The same for the step's gradients, and in one more block the advance of their step counts: the
+// update that follows finds the rates ready, without a launch of their own.
+template <int KIND>
+__global__ __launch_bounds__(THREADS) void norm_advance_kernel(NormTable<ADAM_TENSORS> t, double *partials,
+                                                               StepTable<ADAM_TENSORS> s, int n, AdamArgs a,
+                                                               Rates *rates) {
+    if (blockIdx.x + 1 == gridDim.x) {
+        const int i = threadIdx.x;
+        if (i < n) advance(s.step[i], a, rates + i);
+        return;
+    }
+    norm_partials<KIND>(t, partials, gridDim.x - 1);
+}
+
 template <int KIND> __device__ float norm_of(const double *partials, int n) {
     Running<KIND> r;
     for (int i = threadIdx.x; i < n; i += THREADS) r.join(Running<KIND>::of(partials[i]));
     return block_join(r).value();
+}
+
+// the norm that n partial values make, in every thread of every block that asks
+__device__ inline float norm_of(int kind, const double *partials, int n) {
+    return kind == CISTA_NORM_1   ? norm_of<CISTA_NORM_1>(partials, n)
+           : kind == CISTA_NORM_2 ? norm_of<CISTA_NORM_2>(partials, n)
+                                  : norm_of<CISTA_NORM_MAX>(partials, n);
+}
+
+// Where a kernel takes its norm from: *given, or (given == nullptr) the partial values of the
+// launches before it.  Every block then joins them for itself, in the same order and so to the same
+// bits, and block 0 writes the norm down; that is cheaper than a launch that does it once (22 M
+// float32, 2048 partial values: 143.9 -> 140.7 us for norm and Adam step), but not than one launch
+// for several consumers (200 M bf16 in 5 launches: 1435 -> 1452 us), which get it from a join.
+struct NormSource {
+    const float *given;
+    const double *partials;
+    float *norm;
+    int n, kind;                         // kind 0: no norm
+};
+
+__device__ inline float take_norm(const NormSource &s) {
+    if (s.given) return *s.given;
+    const float v = norm_of(s.kind, s.partials, s.n);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *s.norm = v;
+    return v;
 }
 
 template <int KIND> __global__ __launch_bounds__(THREADS) void norm_join_kernel(const double *partials, int n, float *norm) {
@@ -223,8 +297,8 @@ template <typename T> __device__ void scale_chunk(T *g, uint64_t left, float c) 
 }
 
 // one rounding to the gradient's type, of a float32 product
-__global__ __launch_bounds__(THREADS) void scale_kernel(NormTable t, double max_norm, const float *norm) {
-    const float c = clip_scale(*norm, max_norm);
+__global__ __launch_bounds__(THREADS) void scale_kernel(NormTable<NORM_TENSORS> t, double max_norm, NormSource norm) {
+    const float c = clip_scale(take_norm(norm), max_norm);
     if (c == 1.0f) return;                   // x * 1 is x for every x: nothing to read or write
     const Finder<NORM_TENSORS> find(t.first);
     for (uint32_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
@@ -241,31 +315,6 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(NormTable t, double max_
 }
 
 // ---------------------------------------------------------------------------------- Adam
-struct AdamArgs {
-    double lr, log_beta1, log_beta2, weight_decay, max_norm;
-    const float *lr_device;
-    float rate1, rate2, eps;                 // 1 - b1, 1 - b2
-    float decay;                             // in the gradient; 0 where it is decoupled
-    int decoupled, maximize;
-};
-
-static_assert(sizeof(NormTable) + 32 <= 4096 && sizeof(AdamTable) + sizeof(AdamArgs) + 32 <= 4096, "kernel arguments");
-
-__global__ void adam_advance_kernel(StepTable s, int n, AdamArgs a, Rates *rates) {
-    const int i = threadIdx.x;
-    if (i >= n) return;
-    const float t = *s.step[i] + 1.0f;
-    *s.step[i] = t;
-    const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
-    // 1 - b^t without the cancellation of small t; log(0) = -inf gives 1
-    Rates r;
-    r.size = (float)(lr / -expm1((double)t * a.log_beta1));
-    r.inv_root = (float)(1.0 / sqrt(-expm1((double)t * a.log_beta2)));
-    r.keep = a.decoupled ? (float)(1.0 - lr * a.weight_decay) : 1.0f;
-    r.pad = 0.0f;
-    rates[i] = r;
-}
-
 __device__ inline void adam_element(float &p, float g, float &m, float &v, const AdamArgs &a, const Rates &r, float c) {
     g *= c;
     g = a.maximize ? -g : g;
@@ -305,9 +354,9 @@ __device__ void adam_chunk(T *p, const T *g, float *m, float *v, float *w, uint6
     }
 }
 
-__global__ __launch_bounds__(THREADS) void adam_kernel(AdamTable t, AdamArgs a, const Rates *rates, const float *norm) {
+__global__ __launch_bounds__(THREADS) void adam_kernel(AdamTable t, AdamArgs a, const Rates *rates, NormSource norm) {
     const Finder<ADAM_TENSORS> find(t.first);
-    const float c = norm ? clip_scale(*norm, a.max_norm) : 1.0f;
+    const float c = norm.kind ? clip_scale(take_norm(norm), a.max_norm) : 1.0f;
     for (uint32_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
         const int i = find(k);
         const uint64_t info = t.info[i], off = (uint64_t)(k - t.first[i]) * ADAM_CHUNK;
@@ -387,45 +436,86 @@ int check(const cista_tensor *t, int n, bool written) {
     return overlap(n, [&](int i) { return range_of(t[i].data, t[i].numel, t[i].type); });
 }
 
-// Fills tables of NORM_TENSORS tensors and calls f(table, blocks) for each.
-template <typename Get, typename F> void each_table(int n, Get get, F f) {
-    for (int i = 0; i < n;) {
-        NormTable t;
-        int k = 0;
-        uint64_t chunks = 0;
-        for (; i < n && k < NORM_TENSORS; ++i) {
-            const cista_tensor x = get(i);
-            if (!x.numel) continue;
-            t.data[k] = x.data;
-            t.info[k] = (uint64_t)x.numel | (uint64_t)x.type << 56;
-            t.first[k++] = (uint32_t)chunks;
-            chunks += ((uint64_t)x.numel * size_of(x.type) + NORM_CHUNK - 1) / NORM_CHUNK;
-        }
-        if (!k) break;
-        for (int j = k; j < NORM_TENSORS; ++j) t.data[j] = nullptr, t.info[j] = 0, t.first[j] = ~0u;
-        t.chunks = (uint32_t)chunks;
-        t.pad = 0;
-        f(t, (int)std::min<uint64_t>(chunks, NORM_BLOCKS));
+static_assert(sizeof(NormTable<NORM_TENSORS>) + sizeof(NormSource) + 16 <= 4096, "kernel arguments");
+static_assert(sizeof(AdamTable) + sizeof(AdamArgs) + sizeof(NormSource) + 16 <= 4096, "kernel arguments");
+static_assert(sizeof(NormTable<ADAM_TENSORS>) + sizeof(StepTable<ADAM_TENSORS>) + sizeof(AdamArgs) + 32 <= 4096,
+              "kernel arguments");
+static_assert(sizeof(StepTable<STEP_TENSORS>) + sizeof(AdamArgs) + 16 <= 4096, "kernel arguments");
+
+// The next table of at most N of the n tensors get(i), from i on; i becomes the first one left.
+template <int N, typename Get> NormTable<N> table_of(int &i, int n, Get get) {
+    NormTable<N> t;
+    int k = 0;
+    uint64_t chunks = 0;
+    for (; i < n && k < N; ++i) {
+        const cista_tensor x = get(i);
+        if (!x.numel) continue;
+        t.data[k] = x.data;
+        t.info[k] = (uint64_t)x.numel | (uint64_t)x.type << 56;
+        t.first[k++] = (uint32_t)chunks;
+        chunks += ((uint64_t)x.numel * size_of(x.type) + NORM_CHUNK - 1) / NORM_CHUNK;
     }
+    for (; k < N; ++k) t.data[k] = nullptr, t.info[k] = 0, t.first[k] = ~0u;
+    t.chunks = (uint32_t)chunks;
+    t.pad = 0;
+    return t;
 }
 
-template <int KIND, typename Get> int norm_launch(int n, Get get, float *norm, double *partials, hipStream_t s) {
+int blocks_of(uint32_t chunks, int most) { return (int)std::min<uint32_t>(chunks, most); }
+
+// f(kind as a constant)
+template <typename F> int with_kind(int kind, F f) {
+    switch (kind) {
+    case CISTA_NORM_1: f(std::integral_constant<int, CISTA_NORM_1>()); return CISTA_OK;
+    case CISTA_NORM_2: f(std::integral_constant<int, CISTA_NORM_2>()); return CISTA_OK;
+    case CISTA_NORM_MAX: f(std::integral_constant<int, CISTA_NORM_MAX>()); return CISTA_OK;
+    }
+    return CISTA_ERR_INVALID;
+}
+
+// launches the partial values of all tensors; returns where a norm comes from
+template <typename Get> NormSource partials_of(int kind, int n, Get get, float *norm, double *partials, hipStream_t s) {
     int used = 0;
-    each_table(n, get, [&](const NormTable &t, int blocks) {
-        norm_partials_kernel<KIND><<<blocks, THREADS, 0, s>>>(t, partials + used);
+    for (int i = 0; i < n;) {
+        const auto t = table_of<NORM_TENSORS>(i, n, get);
+        const int blocks = blocks_of(t.chunks, NORM_BLOCKS);
+        if (!blocks) continue;
+        with_kind(kind, [&](auto k) { norm_partials_kernel<k.value><<<blocks, THREADS, 0, s>>>(t, partials + used); });
         used += blocks;
-    });
-    norm_join_kernel<KIND><<<1, THREADS, 0, s>>>(partials, used, norm);
+    }
+    return {nullptr, partials, norm, used, kind};
+}
+
+NormSource join(const NormSource &q, hipStream_t s) {
+    with_kind(q.kind, [&](auto k) { norm_join_kernel<k.value><<<1, THREADS, 0, s>>>(q.partials, q.n, q.norm); });
+    return {q.norm, nullptr, nullptr, 0, q.kind};
+}
+
+int scale(const cista_tensor *grads, int n, double max_norm, NormSource norm, hipStream_t s) {
+    for (int i = 0; i < n;) {
+        const auto t = table_of<NORM_TENSORS>(i, n, [&](int j) { return grads[j]; });
+        const int blocks = blocks_of(t.chunks, NORM_BLOCKS);
+        if (!blocks) continue;
+        scale_kernel<<<blocks, THREADS, 0, s>>>(t, max_norm, norm);
+    }
     return hip_ok();
 }
 
-template <typename Get> int norm_any(int kind, int n, Get get, float *norm, double *partials, hipStream_t s) {
-    switch (kind) {
-    case CISTA_NORM_1: return norm_launch<CISTA_NORM_1>(n, get, norm, partials, s);
-    case CISTA_NORM_2: return norm_launch<CISTA_NORM_2>(n, get, norm, partials, s);
-    case CISTA_NORM_MAX: return norm_launch<CISTA_NORM_MAX>(n, get, norm, partials, s);
-    }
-    return CISTA_ERR_INVALID;
+AdamArgs args_of(const cista_adam_group &q, double max_norm) {
+    AdamArgs a;
+    a.lr = q.lr;
+    a.log_beta1 = std::log(q.beta1);
+    a.log_beta2 = std::log(q.beta2);
+    a.weight_decay = q.weight_decay;
+    a.max_norm = max_norm;
+    a.lr_device = q.lr_device;
+    a.rate1 = (float)(1.0 - q.beta1);
+    a.rate2 = (float)(1.0 - q.beta2);
+    a.eps = (float)q.eps;
+    a.decay = q.decoupled ? 0.0f : (float)q.weight_decay;
+    a.decoupled = q.decoupled;
+    a.maximize = q.maximize;
+    return a;
 }
 
 size_t partial_bytes(int n) { return (size_t)launches(n, NORM_TENSORS) * NORM_BLOCKS * sizeof(double); }
@@ -444,27 +534,32 @@ int cista_grad_norm(const cista_tensor *grads, int n, int norm_kind, float *norm
                     size_t workspace_bytes, void *stream) {
     const int st = check(grads, n, false);
     if (st != CISTA_OK) return st;
-    if (!norm || !workspace) return CISTA_ERR_INVALID;
+    if (!norm || !workspace || norm_kind < CISTA_NORM_1 || norm_kind > CISTA_NORM_MAX) return CISTA_ERR_INVALID;
     if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
-    return norm_any(norm_kind, n, [&](int i) { return grads[i]; }, norm, (double *)workspace, (hipStream_t)stream);
+    hipStream_t s = (hipStream_t)stream;
+    join(partials_of(norm_kind, n, [&](int i) { return grads[i]; }, norm, (double *)workspace, s), s);
+    return hip_ok();
 }
 
 int cista_scale_grads(const cista_tensor *grads, int n, double max_norm, const float *norm, void *stream) {
     const int st = check(grads, n, true);
     if (st != CISTA_OK) return st;
     if (!norm || !(max_norm >= 0.0)) return CISTA_ERR_INVALID;
-    each_table(n, [&](int i) { return grads[i]; }, [&](const NormTable &t, int blocks) {
-        scale_kernel<<<blocks, THREADS, 0, (hipStream_t)stream>>>(t, max_norm, norm);
-    });
-    return hip_ok();
+    return scale(grads, n, max_norm, {norm, nullptr, nullptr, 0, 0}, (hipStream_t)stream);
 }
 
 int cista_clip_grads(const cista_tensor *grads, int n, int norm_kind, double max_norm, float *norm, void *workspace,
                      size_t workspace_bytes, void *stream) {
-    if (!(max_norm >= 0.0)) return CISTA_ERR_INVALID;
-    int st = check(grads, n, true);
-    if (st == CISTA_OK) st = cista_grad_norm(grads, n, norm_kind, norm, workspace, workspace_bytes, stream);
-    return st != CISTA_OK ? st : cista_scale_grads(grads, n, max_norm, norm, stream);
+    const int st = check(grads, n, true);
+    if (st != CISTA_OK) return st;
+    if (!norm || !workspace || norm_kind < CISTA_NORM_1 || norm_kind > CISTA_NORM_MAX || !(max_norm >= 0.0))
+        return CISTA_ERR_INVALID;
+    if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
+    NormSource q = partials_of(norm_kind, n, [&](int i) { return grads[i]; }, norm, (double *)workspace, s);
+    // without partial values (nothing but empty tensors) no other launch would write the norm
+    if (!q.n || n > NORM_TENSORS) q = join(q, s);
+    return scale(grads, n, max_norm, q, s);
 }
 
 int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *groups, int n_groups, int norm_kind,
@@ -501,56 +596,49 @@ int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *grou
     if (!workspace) return CISTA_ERR_INVALID;
     if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
-    if (norm_kind) {
-        const int st = norm_any(norm_kind, n, [&](int i) {
-            return cista_tensor{(void *)table[i].grad, table[i].numel, table[i].type};
-        }, norm, (double *)workspace, s);
-        if (st != CISTA_OK) return st;
-    }
     Rates *rates = (Rates *)((char *)workspace + partial_bytes(n));
+    double *partials = (double *)workspace;
+    const auto grad = [&](int i) { return cista_tensor{(void *)table[i].grad, table[i].numel, table[i].type}; };
+    const bool fused = norm_kind && n_groups == 1 && n <= ADAM_TENSORS;
+    NormSource q = {nullptr, nullptr, nullptr, 0, 0};
+    if (fused) {
+        const AdamArgs a = args_of(groups[0], max_norm);
+        int i = 0;
+        const auto t = table_of<ADAM_TENSORS>(i, n, grad);
+        StepTable<ADAM_TENSORS> steps = {};
+        for (int j = 0; j < n; ++j) steps.step[j] = table[j].step;
+        const int blocks = blocks_of(t.chunks, NORM_BLOCKS);
+        with_kind(norm_kind, [&](auto k) {
+            norm_advance_kernel<k.value><<<blocks + 1, THREADS, 0, s>>>(t, partials, steps, n, a, rates);
+        });
+        q = {nullptr, partials, norm, blocks, norm_kind};
+    } else if (norm_kind) {
+        q = partials_of(norm_kind, n, grad, norm, partials, s);
+    }
+    if (norm_kind && (!q.n || n_groups > 1 || n > ADAM_TENSORS)) q = join(q, s);
     const cista_adam_tensor *x = table;
     for (int k = 0; k < n_groups; ++k) {
-        const cista_adam_group &q = groups[k];
-        AdamArgs a;
-        a.lr = q.lr;
-        a.log_beta1 = std::log(q.beta1);
-        a.log_beta2 = std::log(q.beta2);
-        a.weight_decay = q.weight_decay;
-        a.max_norm = max_norm;
-        a.lr_device = q.lr_device;
-        a.rate1 = (float)(1.0 - q.beta1);
-        a.rate2 = (float)(1.0 - q.beta2);
-        a.eps = (float)q.eps;
-        a.decay = q.decoupled ? 0.0f : (float)q.weight_decay;
-        a.decoupled = q.decoupled;
-        a.maximize = q.maximize;
-        for (int i = 0; i < q.n; i += ADAM_TENSORS) {
-            AdamTable t;
-            StepTable steps;
-            const int now = std::min(ADAM_TENSORS, q.n - i);
+        const AdamArgs a = args_of(groups[k], max_norm);
+        for (int i = 0; !fused && i < groups[k].n; i += STEP_TENSORS) {
+            StepTable<STEP_TENSORS> steps = {};
+            const int now = std::min(STEP_TENSORS, groups[k].n - i);
+            for (int j = 0; j < now; ++j) steps.step[j] = x[i + j].step;
+            adam_advance_kernel<<<1, (now + 63) / 64 * 64, 0, s>>>(steps, now, a, rates + i);
+        }
+        for (int i = 0; i < groups[k].n; i += ADAM_TENSORS) {
+            AdamTable t = {};
+            const int now = std::min(ADAM_TENSORS, groups[k].n - i);
             uint64_t chunks = 0;
-            int used = 0;
-            for (int j = 0; j < ADAM_TENSORS; ++j) {
-                t.param[j] = nullptr, t.grad[j] = nullptr, t.master[j] = nullptr;
-                t.exp_avg[j] = t.exp_avg_sq[j] = nullptr;
-                t.info[j] = 0, t.first[j] = ~0u;
-                steps.step[j] = j < now ? x[j].step : nullptr;
-            }
-            for (int j = 0; j < now; ++j) {
-                t.param[j] = x[j].param, t.grad[j] = x[j].grad, t.master[j] = x[j].master;
-                t.exp_avg[j] = x[j].exp_avg, t.exp_avg_sq[j] = x[j].exp_avg_sq;
-                t.info[j] = (uint64_t)x[j].numel | (uint64_t)x[j].type << 56;
+            for (int j = 0; j < ADAM_TENSORS; ++j) t.first[j] = ~0u;
+            for (int j = 0; j < now; ++j, ++x) {
+                t.param[j] = x->param, t.grad[j] = x->grad, t.master[j] = x->master;
+                t.exp_avg[j] = x->exp_avg, t.exp_avg_sq[j] = x->exp_avg_sq;
+                t.info[j] = (uint64_t)x->numel | (uint64_t)x->type << 56;
                 t.first[j] = (uint32_t)chunks;
-                chunks += ((uint64_t)x[j].numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
-                used = j + 1;
+                chunks += ((uint64_t)x->numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
             }
             t.chunks = (uint32_t)chunks;
-            t.pad = 0;
-            adam_advance_kernel<<<1, ADAM_TENSORS, 0, s>>>(steps, used, a, rates);
-            if (chunks)
-                adam_kernel<<<(int)std::min<uint64_t>(chunks, ADAM_BLOCKS), THREADS, 0, s>>>(t, a, rates,
-                                                                                            norm_kind ? norm : nullptr);
-            x += now;
+            if (chunks) adam_kernel<<<blocks_of(t.chunks, ADAM_BLOCKS), THREADS, 0, s>>>(t, a, rates, q);
             rates += now;
         }
     }
