@@ -18,6 +18,7 @@
  * allocation, no host sync (every call can be captured in a hipGraph), CISTA_* status codes.  The
  * tables of tensors are host arrays, read before the call returns.  A tensor is a dense run of
  * `numel` elements, aligned to its element type only; numel 0 is allowed (data may then be NULL).
+ * One call takes up to 2^40 elements (norm), 68 G (scale, clip) or 17 G (Adam): CISTA_ERR_UNSUPPORTED.
  */
 #ifndef CISTA_OPTIM_H
 #define CISTA_OPTIM_H

@@ -309,7 +309,6 @@ class Adam(torch.optim.Optimizer):
                 if t is not None and p.dtype != torch.float32:
                     self.state[p][name] = t.to(device=p.device, dtype=torch.float32, copy=True)
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -320,6 +319,12 @@ class Adam(torch.optim.Optimizer):
         if norm is not NotImplemented:
             self.grad_norm = norm
             return loss
+        self._step(kind)
+        return loss
+
+    @torch.no_grad()
+    def _step(self, kind):
+        """The step where it is not plain: makes or converts state, copies layouts, refuses."""
         rows, groups, keep, changed = [], [], [], []
         for g in self.param_groups:
             params = [p for p in g["params"] if p.grad is not None]
@@ -351,7 +356,7 @@ class Adam(torch.optim.Optimizer):
             groups.append((lr, g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], lr_device, len(params),
                            int(g["decoupled_weight_decay"]), int(g["maximize"]), 0))
         if not rows:
-            return loss
+            return
         dev = _same_device(changed, "parameters")
         torch.autograd.graph.increment_version(changed)      # the network repacks changed weights
         with _on(dev):
@@ -362,7 +367,6 @@ class Adam(torch.optim.Optimizer):
                 self.max_norm or 0.0, _lib.ptr(norm), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)),
                 "cista_adam_step")
         self.grad_norm = norm
-        return loss
 
 
 class AdamW(Adam):
