@@ -12,7 +12,8 @@
  *
  * The norm is rounded to float32 once (sums run in float64, so squares neither overflow nor
  * vanish); it is NaN if any element is NaN.  A NaN norm makes c NaN, an infinite one makes c 0.
- * Results do not depend on timing: every sum has a fixed order.
+ * Results do not depend on timing: the order of a sum follows from the tensors' sizes and their
+ * places within a 128-byte line.
  *
  * Conventions as in cista_lstc.h: device pointers, `stream` = hipStream_t as void*, no
  * allocation, no host sync (every call can be captured in a hipGraph), CISTA_* status codes.  The

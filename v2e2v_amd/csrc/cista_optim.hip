@@ -22,6 +22,7 @@ constexpr int NORM_TENSORS = 192;        // 20 B each in the kernel argument
 constexpr int NORM_BLOCKS = 2048;        // partial sums of one launch
 constexpr int NORM_UNROLL = 4;           // 16-byte loads in flight per thread
 constexpr int NORM_CHUNK = THREADS * 16 * NORM_UNROLL;                   // bytes
+constexpr int LINE = 128;                // bytes of a cache line
 constexpr int ADAM_TENSORS = 64;         // 52 B each
 constexpr int STEP_TENSORS = 448;        // 8 B each
 constexpr int ADAM_CHUNK = THREADS * 4;  // elements: 4 of a thread
@@ -75,9 +76,11 @@ template <typename T, int V> struct Pack {
 template <int BYTES> struct Words {
     typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(2)));
 };
+#define GLOBAL __attribute__((address_space(1)))
 template <bool STREAM, int V, typename T> __device__ inline Pack<T, V> load(const T *p) {
     using W = typename Words<sizeof(T) * V>::type;
-    const W w = STREAM ? __builtin_nontemporal_load((const W *)p) : *(const W *)p;
+    const GLOBAL W *q = (const GLOBAL W *)p;
+    const W w = STREAM ? __builtin_nontemporal_load(q) : *q;
     Pack<T, V> r;
     __builtin_memcpy(&r, &w, sizeof(r));
     return r;
@@ -86,8 +89,9 @@ template <bool STREAM, typename T, int V> __device__ inline void store(T *p, con
     using W = typename Words<sizeof(T) * V>::type;
     W w;
     __builtin_memcpy(&w, &r, sizeof(w));
-    if (STREAM) __builtin_nontemporal_store(w, (W *)p);
-    else *(W *)p = w;
+    GLOBAL W *q = (GLOBAL W *)p;
+    if (STREAM) __builtin_nontemporal_store(w, q);
+    else *q = w;
 }
 
 // the 16-bit value of a float32 result as it is stored: an opaque register keeps the compiler from
@@ -182,31 +186,52 @@ template <int KIND> __device__ Running<KIND> block_join(Running<KIND> r) {
     return r;
 }
 
-template <int KIND, bool STREAM, typename T>
-__device__ void norm_chunk(Running<KIND> (&acc)[NORM_UNROLL], const T *g, uint64_t left) {
-    constexpr int V = 16 / sizeof(T);
-    const uint32_t at = threadIdx.x * V;
-    if (left >= (uint64_t)NORM_UNROLL * THREADS * V) {
-        Pack<T, V> x[NORM_UNROLL];
-#pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<STREAM, V>(g + at + u * THREADS * V);
-#pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u)
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc[u].add(to_f32(x[u].e[e]));
-        return;
+// A chunk of a tensor for norm and scale: NORM_CHUNK bytes from a cache line's begin, which for the
+// first one may lie before the tensor's.  base: the chunk's first element; [lo, hi): its elements
+// that are the tensor's.
+template <typename T> struct Chunk {
+    static constexpr int V = 16 / sizeof(T), STRIDE = THREADS * V, SIZE = NORM_UNROLL * STRIDE;
+    T *base;
+    int64_t lo, hi;
+    __device__ Chunk(void *data, uint64_t numel, uint32_t chunk) {
+        const uintptr_t at = (uintptr_t)data;
+        const int64_t begin = (int64_t)(at % LINE / sizeof(T)) - (int64_t)chunk * SIZE;
+        base = (T *)data - begin;
+        lo = begin;
+        hi = begin + (int64_t)numel;
     }
-#pragma unroll
-    for (int u = 0; u < NORM_UNROLL; ++u) {
-        const uint32_t i = at + u * THREADS * V;
-        if (i + V <= left) {
-            const Pack<T, V> x = load<STREAM, V>(g + i);
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc[u].add(to_f32(x.e[e]));
-        } else {
-            for (uint32_t e = i; e < left; ++e) acc[u].add(to_f32(g[e]));
+    __device__ bool full() const { return lo <= 0 && hi >= SIZE; }
+    // whole(i) for a thread's vectors that are all the tensor's, one(i) for the elements of the others
+    template <typename F, typename G> __device__ void partly(F whole, G one) const {
+        for (int u = 0; u < NORM_UNROLL; ++u) {
+            const int64_t i = threadIdx.x * V + u * STRIDE;
+            if (i >= lo && i + V <= hi) {
+                whole(u, i);
+            } else {
+                for (int64_t e = i < lo ? lo : i; e < i + V && e < hi; ++e) one(u, e);
+            }
         }
     }
+};
+
+template <int KIND, bool STREAM, typename T>
+__device__ void norm_chunk(Running<KIND> (&acc)[NORM_UNROLL], const Chunk<T> &c) {
+    constexpr int V = Chunk<T>::V;
+    const auto join = [&](int u, const Pack<T, V> &x) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[u].add(to_f32(x.e[e]));
+    };
+    if (c.full()) {
+        const T *g = c.base + threadIdx.x * V;
+        Pack<T, V> x[NORM_UNROLL];
+#pragma unroll
+        for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<STREAM, V>(g + u * c.STRIDE);
+#pragma unroll
+        for (int u = 0; u < NORM_UNROLL; ++u) join(u, x[u]);
+        return;
+    }
+    c.partly([&](int, int64_t i) { join(0, load<STREAM, V>(c.base + i)); },
+             [&](int, int64_t e) { acc[0].add(to_f32(*((const GLOBAL T *)c.base + e))); });
 }
 
 template <int KIND, bool STREAM, int N>
@@ -215,13 +240,12 @@ __device__ void norm_partials(const NormTable<N> &t, double *partials, uint32_t 
     Running<KIND> acc[NORM_UNROLL];
     for (uint32_t c = blockIdx.x; c < t.chunks; c += blocks) {
         const int i = find(c);
-        const uint64_t info = t.info[i], off = (uint64_t)(c - t.first[i]) * NORM_CHUNK;
-        const char *g = (const char *)t.data[i] + off;
-        const uint64_t numel = info & ((1ull << 56) - 1);
-        switch (info >> 56) {
-        case CISTA_F32: norm_chunk<KIND, STREAM>(acc, (const float *)g, numel - off / 4); break;
-        case CISTA_BF16: norm_chunk<KIND, STREAM>(acc, (const __bf16 *)g, numel - off / 2); break;
-        default: norm_chunk<KIND, STREAM>(acc, (const _Float16 *)g, numel - off / 2); break;
+        const uint64_t numel = t.info[i] & ((1ull << 56) - 1);
+        const uint32_t k = c - t.first[i];
+        switch (t.info[i] >> 56) {
+        case CISTA_F32: norm_chunk<KIND, STREAM>(acc, Chunk<float>(t.data[i], numel, k)); break;
+        case CISTA_BF16: norm_chunk<KIND, STREAM>(acc, Chunk<__bf16>(t.data[i], numel, k)); break;
+        default: norm_chunk<KIND, STREAM>(acc, Chunk<_Float16>(t.data[i], numel, k)); break;
         }
     }
 #pragma unroll
@@ -301,22 +325,27 @@ __device__ inline float clip_scale(float norm, double max_norm) {
     return c >= 1.0 ? 1.0f : (float)c;       // a NaN stays one
 }
 
-template <typename T> __device__ void scale_chunk(T *g, uint64_t left, float c) {
-    constexpr int V = 16 / sizeof(T), STRIDE = THREADS * V;
-    if (left >= (uint64_t)NORM_UNROLL * STRIDE) {
+template <typename T> __device__ void scale_chunk(const Chunk<T> &k, float c) {
+    constexpr int V = Chunk<T>::V;
+    const auto scaled = [&](Pack<T, V> x) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x.e[e] = (T)(to_f32(x.e[e]) * c);
+        return x;
+    };
+    if (k.full()) {
+        T *g = k.base + threadIdx.x * V;
         Pack<T, V> x[NORM_UNROLL];
-        g += threadIdx.x * V;
 #pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<false, V>(g + u * STRIDE);
+        for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<false, V>(g + u * k.STRIDE);
 #pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[u].e[e] = (T)(to_f32(x[u].e[e]) * c);
-            store<false>(g + u * STRIDE, x[u]);
-        }
+        for (int u = 0; u < NORM_UNROLL; ++u) store<false>(g + u * k.STRIDE, scaled(x[u]));
         return;
     }
-    for (uint32_t e = threadIdx.x; e < left; e += THREADS) g[e] = (T)(to_f32(g[e]) * c);
+    k.partly([&](int, int64_t i) { store<false>(k.base + i, scaled(load<false, V>(k.base + i))); },
+             [&](int, int64_t e) {
+                 GLOBAL T *g = (GLOBAL T *)k.base + e;
+                 *g = (T)(to_f32(*g) * c);
+             });
 }
 
 // One block per chunk, each rounding once to the gradient's type, of a float32 product.  The chunks
@@ -330,13 +359,12 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(NormTable<NORM_TENSORS> 
     const uint32_t b = blockIdx.x, eights = t.chunks & ~7u;
     const uint32_t k = b < eights ? eights - 8 - (b & ~7u) + (b & 7) : b;
     const int i = find(k);
-    const uint64_t info = t.info[i], off = (uint64_t)(k - t.first[i]) * NORM_CHUNK;
-    char *g = (char *)t.data[i] + off;
-    const uint64_t numel = info & ((1ull << 56) - 1);
-    switch (info >> 56) {
-    case CISTA_F32: scale_chunk((float *)g, numel - off / 4, c); break;
-    case CISTA_BF16: scale_chunk((__bf16 *)g, numel - off / 2, c); break;
-    default: scale_chunk((_Float16 *)g, numel - off / 2, c); break;
+    const uint64_t numel = t.info[i] & ((1ull << 56) - 1);
+    const uint32_t q = k - t.first[i];
+    switch (t.info[i] >> 56) {
+    case CISTA_F32: scale_chunk(Chunk<float>(t.data[i], numel, q), c); break;
+    case CISTA_BF16: scale_chunk(Chunk<__bf16>(t.data[i], numel, q), c); break;
+    default: scale_chunk(Chunk<_Float16>(t.data[i], numel, q), c); break;
     }
 }
 
@@ -355,12 +383,15 @@ __device__ inline void adam_element(float &p, float g, float &m, float &v, const
 }
 
 // Elements [chunk * ADAM_CHUNK - shift, + ADAM_CHUNK) of a tensor, 4 to a thread.  The shift puts the
-// float32 accesses at multiples of 16 bytes where the tensor itself begins between two.
+// float32 accesses on whole cache lines where the tensor itself begins within one, and the 16-bit
+// ones too if they begin at the same element of a line.
+__host__ __device__ inline int64_t adam_shift(const float *m) { return (uintptr_t)m / 4 % (LINE / 2); }
+
 template <bool STREAM, typename T>
 __device__ void adam_chunk(T *p, const T *g, float *m, float *v, float *w, int64_t numel, uint32_t chunk,
                            const AdamArgs &a, const Rates &r, float c) {
     constexpr int V = 4;
-    const int64_t i = (int64_t)chunk * ADAM_CHUNK - (int64_t)((uintptr_t)m / 4 % V) + threadIdx.x * V;
+    const int64_t i = (int64_t)chunk * ADAM_CHUNK - adam_shift(m) + threadIdx.x * V;
     if (i >= 0 && i + V <= numel) {
         const Pack<T, V> gx = load<STREAM, V>(g + i);
         Pack<float, V> wx = load<STREAM, V>(w + i), mx = load<STREAM, V>(m + i), vx = load<STREAM, V>(v + i);
@@ -486,7 +517,7 @@ template <int N, typename Get> NormTable<N> table_of(int &i, int n, Get get) {
         t.data[k] = x.data;
         t.info[k] = (uint64_t)x.numel | (uint64_t)x.type << 56;
         t.first[k++] = (uint32_t)chunks;
-        chunks += ((uint64_t)x.numel * size_of(x.type) + NORM_CHUNK - 1) / NORM_CHUNK;
+        chunks += ((uint64_t)x.numel * size_of(x.type) + (uintptr_t)x.data % LINE + NORM_CHUNK - 1) / NORM_CHUNK;
     }
     for (; k < N; ++k) t.data[k] = nullptr, t.info[k] = 0, t.first[k] = ~0u;
     t.chunks = (uint32_t)chunks;
@@ -676,8 +707,7 @@ int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *grou
                 t.exp_avg[j] = x->exp_avg, t.exp_avg_sq[j] = x->exp_avg_sq;
                 t.info[j] = (uint64_t)x->numel | (uint64_t)x->type << 56;
                 t.first[j] = (uint32_t)chunks;
-                // an element more for each that the shift may move the last one on
-                if (x->numel) chunks += ((uint64_t)x->numel + 3 + ADAM_CHUNK - 1) / ADAM_CHUNK;
+                if (x->numel) chunks += ((uint64_t)x->numel + adam_shift(x->exp_avg) + ADAM_CHUNK - 1) / ADAM_CHUNK;
             }
             t.chunks = (uint32_t)chunks;
             const auto f = stream_all ? adam_kernel<true> : adam_kernel<false>;

@@ -11,7 +11,8 @@ all of its tensors in a few launches, whatever their number, sizes and places in
 
 Types: float32, bfloat16, float16.  Norms are float32, from sums in float64; products are float32,
 rounded once to the gradient's type; moments are float32, and a 16-bit parameter is updated on a
-float32 master copy.  Sums have a fixed order, so equal gradients give equal bits: data-parallel
+float32 master copy.  The order of a sum follows from the tensors' sizes and their places
+within a 128-byte line alone, so equal gradients in equal buffers give equal bits: data-parallel
 replicas stay alike.  Everything runs on the tensors' device, on its current stream, and nothing
 waits for the GPU unless ``error_if_nonfinite`` asks for it, so the calls can be captured into a
 graph.  CPU tensors raise: there is no CPU fallback.
