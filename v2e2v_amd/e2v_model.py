@@ -29,9 +29,22 @@ import weakref
 
 import torch
 import torch.nn as nn
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from . import _lib
 from .base_layers import ConvLayer, ConvLSTC, IstaBlock, RecurrentConvLayer, UpsampleConvLayer
+
+
+def _versions_after_fused_step(optimizer, args, kwargs):
+    """torch's ``fused=True`` optimizers write the parameters without advancing the versions that
+    packed_params and _grad_conduit go by: a network trained with one kept its first packed
+    weights.  This runs after every optimizer step and advances them."""
+    for g in optimizer.param_groups:
+        if g.get("fused"):
+            torch.autograd.graph.increment_version([p for p in g["params"] if p.grad is not None])
+
+
+register_optimizer_step_post_hook(_versions_after_fused_step)
 
 
 class CistaLSTCNet(nn.Module):
