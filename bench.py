@@ -80,15 +80,20 @@ def parse():
                    help="recurrent frames per CPU-baseline sequence (B=1); sequences repeat to ~10 s")
     p.add_argument("--no-cpu-baseline", action="store_true")
     p.add_argument("--layer-reps", type=int, default=10)
-    p.add_argument("--adam", choices=["fused", "foreach"], default="fused",
+    p.add_argument("--adam", choices=["fused", "foreach", "hip"], default="fused",
                    help="--mode train: torch.optim.Adam implementation (the same update; fused = one "
-                        "multi-tensor kernel per step instead of a chain of foreach launches)")
+                        "multi-tensor kernel per step instead of a chain of foreach launches), or hip: "
+                        "v2e2v_amd.optim.Adam")
+    p.add_argument("--max_norm", type=float, default=None,
+                   help="--mode train --adam hip: clip the gradients to this norm within the step")
     p.add_argument("--mode", choices=["infer", "train", "v2e2v"], default="infer",
                    help="infer: the headline metric (config c2); train: BPTT step (configs c3/c4); "
                         "v2e2v: emulator + reconstruction at 720x1280 (config c5)")
     p.add_argument("--num_pack_frames", "--pack-frames", dest="pack_frames", type=int, default=10,
                    help="v2e2v: frames per reconstruction")
     args = p.parse_args()
+    if args.max_norm is not None and (args.mode != "train" or args.adam != "hip"):
+        p.error("--max_norm needs --mode train --adam hip")
     given = lambda *names: any(a in sys.argv for a in names)    # noqa: E731
     if args.mode == "train" and not given("--batch", "--batch_size"):
         args.batch = 8            # BASELINE config c3: batch 8 per GPU (c4: 8 GPUs x 8 = 64)
@@ -283,7 +288,11 @@ def train_main(args, torch, vd, rank, world, device):
         # under torchrun (any N, N=1 included): one bucketed RCCL all-reduce of the gradients
         net = torch.nn.parallel.DistributedDataParallel(model, device_ids=[device.index],
                                                         broadcast_buffers=False)
-    opt = torch.optim.Adam(model.parameters(), lr=1e-4, **({"fused": True} if args.adam == "fused" else {}))
+    if args.adam == "hip":
+        from v2e2v_amd.optim import Adam
+        opt = Adam(model.parameters(), lr=1e-4, max_norm=args.max_norm)
+    else:
+        opt = torch.optim.Adam(model.parameters(), lr=1e-4, **({"fused": True} if args.adam == "fused" else {}))
     vox = synth_voxels(torch, L, B, nb, H, W, args.num_events, seed=2000 + rank, device=device)
     target = torch.rand(B, 1, H, W, device=device, generator=torch.Generator(device=device).manual_seed(3))
 
@@ -335,7 +344,8 @@ def train_main(args, torch, vd, rank, world, device):
                        "batch_per_gpu": B, "global_batch": B * world, "len_sequence": L,
                        "parallelism": f"ddp{world}" if vd.active() else "single",
                        "process_group": (torch.distributed.get_backend() if vd.active() else None),
-                       "optimizer": f"torch.optim.Adam lr 1e-4 ({args.adam})"},
+                       "optimizer": (f"torch.optim.Adam lr 1e-4 ({args.adam})" if args.adam != "hip" else
+                                     f"v2e2v_amd.optim.Adam lr 1e-4, max_norm {args.max_norm}")},
             "loss": float(loss.item()),
             "roofline": roofline, "cpu_baseline": cpu,
             "peak_mem_gb": round(torch.cuda.max_memory_allocated(device) / 1e9, 2)}), flush=True)

@@ -159,3 +159,17 @@ def test_optimizer_object():
 def test_tables_match_the_header():
     assert ctypes.sizeof(optim.CistaTensor) == 24 and ctypes.sizeof(optim.CistaAdamTensor) == 64
     assert ctypes.sizeof(optim.CistaAdamGroup) == 64
+
+
+def test_bench_flags(monkeypatch):
+    """bench.py: --max_norm goes with --mode train --adam hip only."""
+    import sys
+
+    import bench
+    monkeypatch.setattr(sys, "argv", ["bench.py", "--mode", "train", "--adam", "hip", "--max_norm", "0.5"])
+    args = bench.parse()
+    assert args.adam == "hip" and args.max_norm == 0.5
+    for argv in (["--mode", "train", "--max_norm", "0.5"], ["--adam", "hip", "--max_norm", "0.5"]):
+        monkeypatch.setattr(sys, "argv", ["bench.py"] + argv)
+        with pytest.raises(SystemExit):
+            bench.parse()
