@@ -2,7 +2,9 @@
 # runs this Makefile.
 HIPCC ?= /opt/rocm/bin/hipcc
 ARCH  ?= gfx950
-HIPFLAGS = -O3 -std=c++17 --offload-arch=$(ARCH) -fPIC -Wall -Wno-unused-result
+# packed float32 operations stay off: some of their forms have given wrong results on gfx950
+NOPK     = -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS = -O3 -std=c++17 --offload-arch=$(ARCH) -fPIC -Wall -Wno-unused-result $(NOPK)
 
 LIB  = v2e2v_amd/libcista_hip.so
 OBJ  = build/cista_abi.o build/cista_voxel.o build/cista_ssim.o build/cista_v2e.o build/cista_optim.o
@@ -14,6 +16,8 @@ TORCH = $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(
 PYINC = $(shell $(PY) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
 
 all: $(LIB) $(TLIB)
+
+$(OBJ): Makefile
 
 build/cista_abi.o: v2e2v_amd/csrc/cista_abi.hip v2e2v_amd/csrc/cista_kernels.hpp \
                    v2e2v_amd/csrc/cista_backward.hpp include/cista_lstc.h
@@ -32,10 +36,9 @@ build/cista_v2e.o: v2e2v_amd/csrc/cista_v2e.hip include/cista_v2e.h include/cist
 	@mkdir -p build
 	$(HIPCC) $(HIPFLAGS) -c -o $@ $<
 
-# packed float32 operations stay off in this file: some forms have given wrong results on gfx950
 build/cista_optim.o: v2e2v_amd/csrc/cista_optim.hip include/cista_optim.h include/cista_lstc.h
 	@mkdir -p build
-	$(HIPCC) $(HIPFLAGS) -Xclang -target-feature -Xclang -packed-fp32-ops -c -o $@ $<
+	$(HIPCC) $(HIPFLAGS) -c -o $@ $<
 
 $(LIB): $(OBJ)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -o $@ $(OBJ)
