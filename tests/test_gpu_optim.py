@@ -431,6 +431,29 @@ def test_adam_refuses_parameters_that_share_memory():
     assert not base.any()
 
 
+def test_adam_refuses_a_gradient_or_state_of_another_shape():
+    """A parameter that was given other data after its gradient, or its state, was made."""
+    p = torch.nn.Parameter(torch.ones(6, 4, device=DEV))
+    p.grad = torch.ones(6, 4, device=DEV)
+    opt = optim.Adam([p])
+    opt.step()
+    after = p.detach().clone()
+    p.data = after[:, :2].contiguous()
+    with pytest.raises(_lib.CistaError, match="not like its parameter"):
+        opt.step()
+    p.grad = torch.ones(6, 2, device=DEV)
+    with pytest.raises(_lib.CistaError, match="state exp_avg has shape"):
+        opt.step()
+    p.data = after.t().contiguous()                       # as many elements, other places
+    p.grad = torch.ones(4, 6, device=DEV)
+    with pytest.raises(_lib.CistaError, match="state exp_avg has shape"):
+        opt.step()
+    p.data = after.bfloat16()
+    p.grad = torch.ones(6, 4, device=DEV, dtype=torch.bfloat16)
+    opt.step()                                            # another type: a master copy is made
+    assert opt.state[p]["master"].dtype == torch.float32 and opt.state[p]["step"].item() == 2
+
+
 def test_adam_of_zero_gradients_and_overflowing_squares():
     p = torch.nn.Parameter(torch.ones(5000, device=DEV))
     p.grad = torch.zeros_like(p)

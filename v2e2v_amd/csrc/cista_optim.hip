@@ -201,37 +201,38 @@ template <typename T> struct Chunk {
         hi = begin + (int64_t)numel;
     }
     __device__ bool full() const { return lo <= 0 && hi >= SIZE; }
-    // whole(i) for a thread's vectors that are all the tensor's, one(i) for the elements of the others
-    template <typename F, typename G> __device__ void partly(F whole, G one) const {
-        for (int u = 0; u < NORM_UNROLL; ++u) {
-            const int64_t i = threadIdx.x * V + u * STRIDE;
-            if (i >= lo && i + V <= hi) {
-                whole(u, i);
-            } else {
-                for (int64_t e = i < lo ? lo : i; e < i + V && e < hi; ++e) one(u, e);
-            }
+    // a thread's vector u, and whether all of it is the tensor's
+    __device__ int64_t at(int u) const { return threadIdx.x * V + u * STRIDE; }
+    __device__ bool inside(int u) const { return at(u) >= lo && at(u) + V <= hi; }
+    // the thread's vectors; zeros for those that are not inside.  All loads are under way at once,
+    // also at a tensor's ends: a small tensor is nothing else.
+    template <bool STREAM> __device__ void read(Pack<T, V> (&x)[NORM_UNROLL]) const {
+        if (full()) {
+#pragma unroll
+            for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<STREAM, V>(base + at(u));
+        } else {
+#pragma unroll
+            for (int u = 0; u < NORM_UNROLL; ++u) x[u] = inside(u) ? load<STREAM, V>(base + at(u)) : Pack<T, V>{};
         }
+    }
+    // f(element) for the tensor's elements in the thread's other vectors
+    template <typename F> __device__ void ends(F f) const {
+        if (full()) return;
+        for (int u = 0; u < NORM_UNROLL; ++u)
+            if (!inside(u))
+                for (int64_t e = at(u) < lo ? lo : at(u); e < at(u) + V && e < hi; ++e) f(*((GLOBAL T *)base + e));
     }
 };
 
 template <int KIND, bool STREAM, typename T>
 __device__ void norm_chunk(Running<KIND> (&acc)[NORM_UNROLL], const Chunk<T> &c) {
-    constexpr int V = Chunk<T>::V;
-    const auto join = [&](int u, const Pack<T, V> &x) {
+    Pack<T, Chunk<T>::V> x[NORM_UNROLL];
+    c.template read<STREAM>(x);
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[u].add(to_f32(x.e[e]));
-    };
-    if (c.full()) {
-        const T *g = c.base + threadIdx.x * V;
-        Pack<T, V> x[NORM_UNROLL];
+    for (int u = 0; u < NORM_UNROLL; ++u)
 #pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<STREAM, V>(g + u * c.STRIDE);
-#pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u) join(u, x[u]);
-        return;
-    }
-    c.partly([&](int, int64_t i) { join(0, load<STREAM, V>(c.base + i)); },
-             [&](int, int64_t e) { acc[0].add(to_f32(*((const GLOBAL T *)c.base + e))); });
+        for (int e = 0; e < c.V; ++e) acc[u].add(to_f32(x[u].e[e]));
+    c.ends([&](GLOBAL T &g) { acc[0].add(to_f32(g)); });
 }
 
 template <int KIND, bool STREAM, int N>
@@ -326,26 +327,15 @@ __device__ inline float clip_scale(float norm, double max_norm) {
 }
 
 template <typename T> __device__ void scale_chunk(const Chunk<T> &k, float c) {
-    constexpr int V = Chunk<T>::V;
-    const auto scaled = [&](Pack<T, V> x) {
+    Pack<T, Chunk<T>::V> x[NORM_UNROLL];
+    k.template read<false>(x);
 #pragma unroll
-        for (int e = 0; e < V; ++e) x.e[e] = (T)(to_f32(x.e[e]) * c);
-        return x;
-    };
-    if (k.full()) {
-        T *g = k.base + threadIdx.x * V;
-        Pack<T, V> x[NORM_UNROLL];
+    for (int u = 0; u < NORM_UNROLL; ++u) {
 #pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u) x[u] = load<false, V>(g + u * k.STRIDE);
-#pragma unroll
-        for (int u = 0; u < NORM_UNROLL; ++u) store<false>(g + u * k.STRIDE, scaled(x[u]));
-        return;
+        for (int e = 0; e < k.V; ++e) x[u].e[e] = (T)(to_f32(x[u].e[e]) * c);
+        if (k.full() || k.inside(u)) store<false>(k.base + k.at(u), x[u]);
     }
-    k.partly([&](int, int64_t i) { store<false>(k.base + i, scaled(load<false, V>(k.base + i))); },
-             [&](int, int64_t e) {
-                 GLOBAL T *g = (GLOBAL T *)k.base + e;
-                 *g = (T)(to_f32(*g) * c);
-             });
+    k.ends([&](GLOBAL T &g) { g = (T)(to_f32(g) * c); });
 }
 
 // One block per chunk, each rounding once to the gradient's type, of a float32 product.  The chunks

@@ -335,9 +335,9 @@ class Adam(torch.optim.Optimizer):
                 _check_tensor(grad, "gradient")
                 if not _dense(p):
                     raise _lib.CistaError(f"a parameter of strides {p.stride()} does not fill its memory")
-                if grad.dtype != p.dtype or grad.device != p.device:
-                    raise _lib.CistaError(f"a gradient ({grad.dtype}, {grad.device}) is not like its parameter "
-                                          f"({p.dtype}, {p.device})")
+                if grad.shape != p.shape or grad.dtype != p.dtype or grad.device != p.device:
+                    raise _lib.CistaError(f"a gradient ({tuple(grad.shape)}, {grad.dtype}, {grad.device}) is not like its "
+                                          f"parameter ({tuple(p.shape)}, {p.dtype}, {p.device})")
                 if grad.stride() != p.stride() and not (grad.is_contiguous() and p.is_contiguous()):
                     grad = torch.empty_like(p, requires_grad=False).copy_(grad)
                     keep.append(grad)
@@ -357,6 +357,7 @@ class Adam(torch.optim.Optimizer):
             groups.append((lr, g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], lr_device, len(params),
                            int(g["decoupled_weight_decay"]), int(g["maximize"]), 0))
         if not rows:
+            self.grad_norm = None
             return
         dev = _same_device(changed, "parameters")
         torch.autograd.graph.increment_version(changed)      # the network repacks changed weights
