@@ -615,6 +615,41 @@ def test_a_run_taken_up_again():
         assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+@pytest.mark.parametrize("kw", [{}, {"foreach": True}, {"fused": True}])
+def test_state_of_torchs_optimizer(kw):
+    """A run is taken up from torch.optim.Adam's state_dict, and given back to it."""
+    def grads(ps, k):
+        for i, p in enumerate(ps):
+            p.grad = torch.randn(p.shape, device=DEV, generator=gen(50 * k + i))
+
+    ps, qs = (adam_case([3, 4000], torch.float32, 95, 0)[0] for _ in range(2))
+    other, own = torch.optim.Adam(ps, lr=1e-2, **kw), optim.Adam(qs, lr=7.0)
+    for k in range(3):
+        grads(ps, k)
+        other.step()
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+    own.load_state_dict(other.state_dict())
+    hyper = dict(HYPER, lr=1e-2)
+    grads(qs, 3)
+    before = snapshot(own, qs, {})
+    own.step()
+    check_step(own, qs, before, hyper, 4, 1.0)
+    back = torch.optim.Adam(ps, lr=5.0, **kw)
+    back.load_state_dict(own.state_dict())
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            p.copy_(q)
+    grads(ps, 4)
+    before = [(p.detach().clone(), back.state[p]["exp_avg"].clone(), back.state[p]["exp_avg_sq"].clone()) for p in ps]
+    back.step()
+    for p, (w, m, v) in zip(ps, before):
+        # the other optimizer orders its operations in its own way: a few roundings more
+        w1, m1, v1, (ew, em, ev) = adam64(w, p.grad, m, v, 5, 1.0, **hyper)
+        assert back.state[p]["step"].item() == 5 and bool(((p.detach().double() - w1).abs() <= 4 * ew).all())
+
+
 def test_offsets_past_32_bits():
     """Norm, clipping and the step on tensors whose byte and element offsets pass 32 bits."""
     n = 2 ** 32 + 4099

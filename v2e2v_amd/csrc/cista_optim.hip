@@ -188,7 +188,8 @@ template <int KIND> __device__ Running<KIND> block_join(Running<KIND> r) {
 
 // A chunk of a tensor for norm and scale: NORM_CHUNK bytes from a cache line's begin, which for the
 // first one may lie before the tensor's.  base: the chunk's first element; [lo, hi): its elements
-// that are the tensor's.
+// that are the tensor's.  Cut at the tensor's begin instead, a bf16 tensor at an odd 2-byte place is
+// read at 5.2 TB/s, one at an odd 16 bytes at 6.7; cut so, at 6.9 wherever it begins (1.2 GB).
 template <typename T> struct Chunk {
     static constexpr int V = 16 / sizeof(T), STRIDE = THREADS * V, SIZE = NORM_UNROLL * STRIDE;
     T *base;
@@ -374,7 +375,8 @@ __device__ inline void adam_element(float &p, float g, float &m, float &v, const
 
 // Elements [chunk * ADAM_CHUNK - shift, + ADAM_CHUNK) of a tensor, 4 to a thread.  The shift puts the
 // float32 accesses on whole cache lines where the tensor itself begins within one, and the 16-bit
-// ones too if they begin at the same element of a line.
+// ones too if they begin at the same element of a line (AdamW with clipping of 268 M float32 in 147
+// tensors end to end 1515 -> 1428 us, of 200 M bf16 in 301 tensors 1115 -> 1005 us).
 __host__ __device__ inline int64_t adam_shift(const float *m) { return (uintptr_t)m / 4 % (LINE / 2); }
 
 template <bool STREAM, typename T>
@@ -404,11 +406,13 @@ __device__ void adam_chunk(T *p, const T *g, float *m, float *v, float *w, int64
     }
 }
 
-// One block per chunk, dispatched in the order of the addresses: a grid of 2048 blocks that step
-// through the chunks drifts apart over the seven streams and loses the DRAM's pages (268 M float32
-// without clipping: 1632 us, one block per chunk 1404 us, with STREAM 1358 us = 5.5 TB/s, where a
-// 4 GiB copy reaches 4.9).  Where all of it fits the last-level cache STREAM costs (1.4 M parameters:
-// 8.5 -> 9.5 us), so it goes by the bytes.
+// Seven streams over HBM, 28 bytes and some 40 operations an element: bound by HBM (268 M float32:
+// 1259 us, 6.0 TB/s, where a 4 GiB copy reaches 4.9), or by launches where it is small.  One block
+// per chunk, dispatched in the order of the addresses: 2048 blocks that step through the chunks drift
+// apart and lose the DRAM's pages (1632 us against 1404, before the lines and STREAM).  Where all of it
+// fits the last-level cache STREAM costs (1.4 M parameters: 8.5 -> 9.5 us; 268 M: 1404 -> 1358), so
+// it goes by the bytes.  The blocks of an XCD (block mod 8) take the chunks whose gradients its L2
+// has from the norm: 4 of them to a chunk of the norm's.
 template <bool STREAM>
 __global__ __launch_bounds__(THREADS) void adam_kernel(AdamTable t, AdamArgs a, const Rates *rates, NormSource norm) {
     const Finder<ADAM_TENSORS> find(t.first);
