@@ -39,7 +39,7 @@ typedef struct {
     long long type;          /* CISTA_F32 / _BF16 / _F16                                          */
 } cista_tensor;
 
-/* workspace of every call below, for n tensors */
+/* workspace of every call below, for n tensors; 16-byte aligned, used by one call at a time */
 size_t cista_optim_workspace_bytes(int n);
 
 /* *norm = the norm of the n tensors (float32, device); n = 0 gives 0 */

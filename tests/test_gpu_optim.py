@@ -234,6 +234,8 @@ def test_clipping_of_nonfinite_norms():
     assert g[:2].tolist() == [0.0, 0.0] and math.isnan(g[2].item())
     g = torch.tensor([1.0, -2.0, math.nan], device=DEV, dtype=torch.float16)
     assert math.isnan(optim.clip_grad_norm_(params_of([g]), 1.0).item()) and bool(g.isnan().all())
+    g = torch.tensor([1.0, -2.0, math.nan] + [3.0] * 5000, device=DEV, dtype=torch.bfloat16)
+    assert math.isnan(optim.clip_grad_norm_(params_of([g]), 1.0).item()) and bool(g.isnan().all())
     g = torch.tensor([1.0, -2.0, math.inf], device=DEV, dtype=torch.bfloat16)
     optim.clip_grad_norm_(params_of([g]), math.inf)                                   # no limit: nothing is scaled
     assert g.tolist() == [1.0, -2.0, math.inf]
@@ -536,6 +538,27 @@ def test_side_streams_at_once():
     for i in range(2):
         assert all(abs(n.item() - want[i]) <= SPARE * U * want[i] for n in norms[i])
         check_scaled(sets[i], old[i], 1.0 / (want[i] + 1e-6))
+
+
+def test_steps_on_a_side_stream():
+    """A stream of its own, gradients made on it, and memory freed and reused between the steps."""
+    torch.cuda.synchronize()
+    runs = []
+    for s in (torch.cuda.Stream(), torch.cuda.current_stream()):
+        with torch.cuda.stream(s):
+            ps, _ = adam_case([70001, 3, 500000], torch.bfloat16, 65, 0)
+            opt = optim.AdamW(ps, lr=1e-2, max_norm=0.5)
+            for k in range(6):
+                for i, p in enumerate(ps):
+                    p.grad = torch.randn(p.shape, device=DEV, generator=gen(10 * k + i)).bfloat16()
+                opt.step()
+                del p
+                spill = torch.full((1 << 20,), math.nan, device=DEV)    # what a freed workspace may become
+                del spill
+            s.synchronize()
+            runs.append([p.detach().clone() for p in ps] + [opt.grad_norm])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
 def test_captured_steps_replay_like_eager_ones():

@@ -41,6 +41,10 @@ def test_c_entries_refuse_bad_tables():
     assert L.cista_grad_norm(table(ok), 1, 4, FAKE, FAKE, big, None) == 1
     assert L.cista_grad_norm(table(ok), 1, 2, None, FAKE, big, None) == 1
     assert L.cista_grad_norm(table(ok), 1, 2, FAKE, None, big, None) == 1
+    assert L.cista_grad_norm(table(ok), 1, 2, FAKE + 2, FAKE, big, None) == 1           # misaligned
+    assert L.cista_grad_norm(table(ok), 1, 2, FAKE, FAKE + 8, big, None) == 1
+    assert L.cista_scale_grads(table(ok), 1, 1.0, FAKE + 1, None) == 1
+    assert L.cista_clip_grads(table(ok), 1, 2, 1.0, FAKE, FAKE + 4, big, None) == 1
     need = L.cista_optim_workspace_bytes(1)
     assert L.cista_grad_norm(table(ok), 1, 2, FAKE, FAKE, need - 1, None) == 4
     assert L.cista_clip_grads(table(ok), 1, 2, 1.0, FAKE, FAKE, need - 1, None) == 4
@@ -77,6 +81,15 @@ def test_adam_entry_refuses():
     assert adam_call([adam_row(kind=1)]) == 1           # 16 bits without a master copy
     assert adam_call([adam_row(), adam_row(param=FAKE + 60)]) == 5
     assert adam_call([adam_row()], ws=None) == 1
+    assert adam_call([adam_row()], ws=FAKE + 8) == 1
+    assert adam_call([adam_row(step=FAKE + 2)]) == 1
+    assert adam_call([adam_row()], group=(1e-3, 0.9, 0.9, 1e-8, 0.0, FAKE + 2, 1, 0, 0, 0)) == 1
+    twice = [adam_row(), adam_row(param=9 * FAKE, grad=9 * FAKE, m=10 * FAKE, v=11 * FAKE, step=12 * FAKE)]
+    for k in (2, 3, 5):                                  # the same m, v or step for two parameters
+        rows = [twice[0], tuple(twice[0][j] if j == k else x for j, x in enumerate(twice[1]))]
+        assert adam_call(rows) == 5
+    half = [adam_row(master=6 * FAKE, kind=1), adam_row(9 * FAKE, 9 * FAKE, 10 * FAKE, 11 * FAKE, 6 * FAKE + 4, 12 * FAKE, kind=1)]
+    assert adam_call(half) == 5
     assert adam_call([adam_row()], nbytes=need - 1) == 4
     assert adam_call([adam_row()], norm_kind=4, norm=FAKE) == 1
     assert adam_call([adam_row()], norm_kind=2, norm=None) == 1

@@ -448,6 +448,10 @@ bool bad_tensor(const void *data, long long numel, long long type) {
     return numel > 0 && (!data || (uintptr_t)data % size_of(type));
 }
 
+// how a float is aligned, and what the partial values and rates need
+bool misplaced(const float *x) { return (uintptr_t)x % sizeof(float); }
+bool misplaced(const void *workspace) { return (uintptr_t)workspace % 16; }
+
 struct Range {
     uintptr_t begin, end;
 };
@@ -606,7 +610,9 @@ int cista_grad_norm(const cista_tensor *grads, int n, int norm_kind, float *norm
                     size_t workspace_bytes, void *stream) {
     const int st = check(grads, n, false);
     if (st != CISTA_OK) return st;
-    if (!norm || !workspace || norm_kind < CISTA_NORM_1 || norm_kind > CISTA_NORM_MAX) return CISTA_ERR_INVALID;
+    if (!norm || !workspace || norm_kind < CISTA_NORM_1 || norm_kind > CISTA_NORM_MAX || misplaced(norm) ||
+        misplaced(workspace))
+        return CISTA_ERR_INVALID;
     if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     // past the cache's size nobody finds the gradients there anyway (1.2 GB of bf16: 212 -> 199 us)
@@ -619,7 +625,7 @@ int cista_grad_norm(const cista_tensor *grads, int n, int norm_kind, float *norm
 int cista_scale_grads(const cista_tensor *grads, int n, double max_norm, const float *norm, void *stream) {
     const int st = check(grads, n, true);
     if (st != CISTA_OK) return st;
-    if (!norm || !(max_norm >= 0.0)) return CISTA_ERR_INVALID;
+    if (!norm || misplaced(norm) || !(max_norm >= 0.0)) return CISTA_ERR_INVALID;
     return scale(grads, n, max_norm, {norm, nullptr, nullptr, 0, 0}, (hipStream_t)stream);
 }
 
@@ -627,7 +633,8 @@ int cista_clip_grads(const cista_tensor *grads, int n, int norm_kind, double max
                      size_t workspace_bytes, void *stream) {
     const int st = check(grads, n, true);
     if (st != CISTA_OK) return st;
-    if (!norm || !workspace || norm_kind < CISTA_NORM_1 || norm_kind > CISTA_NORM_MAX || !(max_norm >= 0.0))
+    if (!norm || !workspace || norm_kind < CISTA_NORM_1 || norm_kind > CISTA_NORM_MAX || !(max_norm >= 0.0) ||
+        misplaced(norm) || misplaced(workspace))
         return CISTA_ERR_INVALID;
     if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
@@ -640,18 +647,20 @@ int cista_clip_grads(const cista_tensor *grads, int n, int norm_kind, double max
 int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *groups, int n_groups, int norm_kind,
                     double max_norm, float *norm, void *workspace, size_t workspace_bytes, void *stream) {
     if (n_groups < 0 || (n_groups && !groups) || norm_kind < 0 || norm_kind > CISTA_NORM_MAX) return CISTA_ERR_INVALID;
-    if (norm_kind && (!norm || !(max_norm >= 0.0))) return CISTA_ERR_INVALID;
+    if (norm_kind && (!norm || misplaced(norm) || !(max_norm >= 0.0))) return CISTA_ERR_INVALID;
     int n = 0;
     for (int k = 0; k < n_groups; ++k) {
         const cista_adam_group &q = groups[k];
-        if (q.n < 0 || !(q.beta1 >= 0.0 && q.beta1 < 1.0 && q.beta2 >= 0.0 && q.beta2 < 1.0)) return CISTA_ERR_INVALID;
+        if (q.n < 0 || !(q.beta1 >= 0.0 && q.beta1 < 1.0 && q.beta2 >= 0.0 && q.beta2 < 1.0) ||
+            misplaced(q.lr_device))
+            return CISTA_ERR_INVALID;
         n += q.n;
     }
     if (n && !table) return CISTA_ERR_INVALID;
     long long total = 0;
     for (int i = 0; i < n; ++i) {
         const cista_adam_tensor &x = table[i];
-        if (bad_tensor(x.param, x.numel, x.type) || bad_tensor(x.grad, x.numel, x.type) || !x.step ||
+        if (bad_tensor(x.param, x.numel, x.type) || bad_tensor(x.grad, x.numel, x.type) || !x.step || misplaced(x.step) ||
             bad_tensor(x.exp_avg, x.numel, CISTA_F32) || bad_tensor(x.exp_avg_sq, x.numel, CISTA_F32) ||
             (x.type != CISTA_F32 && bad_tensor(x.master, x.numel, CISTA_F32)))
             return CISTA_ERR_INVALID;
@@ -668,7 +677,7 @@ int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *grou
         });
     }
     if (apart != CISTA_OK) return apart;
-    if (!workspace) return CISTA_ERR_INVALID;
+    if (!workspace || misplaced(workspace)) return CISTA_ERR_INVALID;
     if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     Rates *rates = (Rates *)((char *)workspace + partial_bytes(n));
