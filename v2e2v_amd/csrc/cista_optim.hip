@@ -19,7 +19,7 @@ namespace cista_optim {
 
 constexpr int THREADS = 256;
 constexpr int NORM_TENSORS = 192;        // 20 B each in the kernel argument
-constexpr int NORM_BLOCKS = 2048;        // partial sums of one launch
+constexpr int NORM_BLOCKS = 1024;        // partial sums of one launch: the blocks that run at once (92 VGPRs)
 constexpr int NORM_UNROLL = 4;           // 16-byte loads in flight per thread
 constexpr int NORM_CHUNK = THREADS * 16 * NORM_UNROLL;                   // bytes
 constexpr int LINE = 128;                // bytes of a cache line
@@ -28,6 +28,7 @@ constexpr int STEP_TENSORS = 448;        // 8 B each
 constexpr int ADAM_CHUNK = THREADS * 4;  // elements: 4 of a thread
 constexpr int JOIN_ALL = 512;            // partial values that every block of the next launch joins
 constexpr long long CACHE = 256ll << 20; // bytes of the last-level cache
+constexpr int FIVE = 32000;              // bytes of LDS with which 5 blocks run on a CU
 
 // chunk c belongs to the last tensor whose first chunk is <= c (unused entries: ~0u; an empty
 // tensor's first chunk is the next one's, which is found in its place)
@@ -236,6 +237,9 @@ __device__ void norm_chunk(Running<KIND> (&acc)[NORM_UNROLL], const Chunk<T> &c)
     c.ends([&](GLOBAL T &g) { acc[0].add(to_f32(g)); });
 }
 
+// Bound by HBM reads (600 M bf16: 186 us, 6.5 TB/s), or for few elements by the latency of a launch and
+// its join.  A block steps through the chunks; 2048 blocks, half of which wait for a place, take 189 us
+// and leave twice as many values to join (22 M float32, norm and scale: 39 -> 42 us).
 template <int KIND, bool STREAM, int N>
 __device__ void norm_partials(const NormTable<N> &t, double *partials, uint32_t blocks) {
     const Finder<N> find(t.first);
@@ -407,12 +411,14 @@ __device__ void adam_chunk(T *p, const T *g, float *m, float *v, float *w, int64
 }
 
 // Seven streams over HBM, 28 bytes and some 40 operations an element: bound by HBM (268 M float32:
-// 1259 us, 6.0 TB/s, where a 4 GiB copy reaches 4.9), or by launches where it is small.  One block
+// 1195 us, 6.3 TB/s, where a 4 GiB copy reaches 4.9), or by launches where it is small.  One block
 // per chunk, dispatched in the order of the addresses: 2048 blocks that step through the chunks drift
 // apart and lose the DRAM's pages (1632 us against 1404, before the lines and STREAM).  Where all of it
 // fits the last-level cache STREAM costs (1.4 M parameters: 8.5 -> 9.5 us; 268 M: 1404 -> 1358), so
-// it goes by the bytes.  The blocks of an XCD (block mod 8) take the chunks whose gradients its L2
-// has from the norm: 4 of them to a chunk of the norm's.
+// it goes by the bytes, and so does FIVE: with 5 blocks on a CU instead of 8 the blocks stay closer
+// together (1249 -> 1195 us, 6.3 TB/s; 3 blocks 1237; 1.4 M parameters: 9.0 -> 9.3 us).  The blocks of an
+// XCD (block mod 8) take the chunks whose gradients its L2 has from the norm: 4 of them to a chunk of
+// the norm's.
 template <bool STREAM>
 __global__ __launch_bounds__(THREADS) void adam_kernel(AdamTable t, AdamArgs a, const Rates *rates, NormSource norm) {
     const Finder<ADAM_TENSORS> find(t.first);
@@ -724,7 +730,7 @@ int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *grou
             }
             t.chunks = (uint32_t)chunks;
             const auto f = stream_all ? adam_kernel<true> : adam_kernel<false>;
-            if (chunks) f<<<t.chunks, THREADS, 0, s>>>(t, a, rates, q);
+            if (chunks) f<<<t.chunks, THREADS, stream_all ? FIVE : 0, s>>>(t, a, rates, q);
             rates += now;
         }
     }
