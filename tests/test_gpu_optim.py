@@ -228,6 +228,37 @@ def params_of_views(grads):
     return out
 
 
+def test_gradients_that_are_odd_views():
+    """A gradient that repeats one element is refused before anything is written; a lazily negated one counts
+    with its sign."""
+    ps = params_of([torch.ones(4, device=DEV)]) + params_of_views([torch.ones(1, device=DEV).expand(6)])
+    with pytest.raises(_lib.CistaError, match="overlaps itself"):
+        optim.clip_grad_norm_(ps, 1e-3)
+    with pytest.raises(_lib.CistaError, match="overlaps itself"):
+        optim.clip_grads_with_norm_(ps, 1e-3, torch.tensor(1.0, device=DEV))
+    assert torch.equal(ps[0].grad, torch.ones(4, device=DEV))
+    near(optim.grad_norm([p.grad for p in ps]), math.sqrt(10.0), 2)
+    z = torch.complex(torch.randn(50, device=DEV, generator=gen(2)), torch.randn(50, device=DEV, generator=gen(3)))
+    neg = z.conj().imag
+    assert neg.is_neg()
+    p = params_of_views([neg])[0]
+    old, hyper = neg.clone(), dict(HYPER)
+    opt = make([p], {}, hyper)
+    before = snapshot(opt, [p], {})
+    opt.step()
+    check_step(opt, [p], before, hyper, 1, 1.0)
+    norm = norm64([old], 2)
+    near(optim.clip_grad_norm_([p], 0.5), norm, 2)
+    check_scaled([p.grad.clone()], [old], 0.5 / (norm + 1e-6))
+    flat = torch.view_as_real(z)[:, 1].neg().contiguous()._neg_view()       # dense, and negated
+    q = params_of([torch.zeros(50, device=DEV)])[0]
+    q.grad = flat
+    opt = make([q], {}, hyper)
+    before = snapshot(opt, [q], {})
+    opt.step()
+    check_step(opt, [q], before, hyper, 1, 1.0)
+
+
 def test_clipping_of_nonfinite_norms():
     g = torch.tensor([1.0, -2.0, math.inf], device=DEV)
     assert optim.clip_grad_norm_(params_of([g]), 1.0).item() == math.inf

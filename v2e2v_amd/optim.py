@@ -167,6 +167,8 @@ def _written(grads, call):
 def _check_grads(grads):
     for g in grads:
         _check_tensor(g, "gradient")
+        if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+            raise _lib.CistaError(f"a gradient of strides {g.stride()} overlaps itself and cannot be written")
     return _same_device(grads, "gradients")
 
 
@@ -333,12 +335,13 @@ class Adam(torch.optim.Optimizer):
                 _check_tensor(p, "parameter")
                 grad = p.grad
                 _check_tensor(grad, "gradient")
-                if not _dense(p):
+                if not _dense(p):                         # a negated view is none
                     raise _lib.CistaError(f"a parameter of strides {p.stride()} does not fill its memory")
                 if grad.shape != p.shape or grad.dtype != p.dtype or grad.device != p.device:
                     raise _lib.CistaError(f"a gradient ({tuple(grad.shape)}, {grad.dtype}, {grad.device}) is not like its "
                                           f"parameter ({tuple(p.shape)}, {p.dtype}, {p.device})")
-                if grad.stride() != p.stride() and not (grad.is_contiguous() and p.is_contiguous()):
+                if grad.is_neg() or (
+                        grad.stride() != p.stride() and not (grad.is_contiguous() and p.is_contiguous())):
                     grad = torch.empty_like(p, requires_grad=False).copy_(grad)
                     keep.append(grad)
                 st = self._slot(p)
