@@ -1,0 +1,68 @@
+"""Places where the training-step operators (v2e2v_amd/optim.py) lose what the formula keeps, or take what
+they should refuse: small decay rates of the moments, a 16-bit value's one rounding, small decoupled decay,
+state that outlives its parameter's type, views that share memory, and tensors past the cache's size.
+
+U = 2^-24 is half a step of float32 relative to the value; the helpers and the two ways that each test
+takes are those of tests/test_gpu_optim.py.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_optim import (DEV, HYPER, ODD, SPARE, TYPES, U, adam_bounds, adam_case, check_scaled, check_step, gen,  # noqa: F401
+                                  make, near, norm64, params_of, params_of_views, snapshot, some, way)
+from v2e2v_amd import _lib, optim
+
+pytestmark = pytest.mark.gpu
+
+
+# ----------------------------------------------------------------------------- moments of small rates
+def wide_case(dtype, seed):
+    """Gradients over nine orders of magnitude beside moments of about 1."""
+    ps = []
+    for i, n in enumerate((1, 5, 1023, 4097)):
+        p = torch.nn.Parameter((torch.rand(n, device=DEV, generator=gen(seed + i)) + 0.5).to(dtype))
+        mag = 10.0 ** (-9.0 * torch.rand(n, device=DEV, generator=gen(seed + 10 + i), dtype=torch.float64))
+        p.grad = (mag * torch.randn(n, device=DEV, generator=gen(seed + 20 + i)).sign()).to(dtype)
+        ps.append(p)
+    state = {i: dict(step=torch.tensor(3.0), exp_avg=torch.randn(p.shape, device=DEV, generator=gen(seed + 30 + i)),
+                     exp_avg_sq=torch.rand(p.shape, device=DEV, generator=gen(seed + 40 + i)),
+                     **({} if dtype == torch.float32 else {"master": p.detach().float()})) for i, p in enumerate(ps)}
+    return ps, state
+
+
+@pytest.mark.parametrize("b1", [0.0, 1e-9, 0.1, 0.3, 0.49])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_first_moment_of_a_small_beta1(dtype, b1):
+    """The old moment counts with b1, its roundings too.  b1 m + (1 - b1) g: b1, its product's sum and 1 - b1 are
+    off by U each, the product (1 - b1) g too, and the sum by U of the result:
+    U (2 b1 |m| + 3 (1 - b1) |g|), plus half of the smallest number for each of two results."""
+    ps, state = wide_case(dtype, 7)
+    opt = make(ps, state, dict(HYPER, betas=(b1, 0.999)))
+    before = snapshot(opt, ps, state)
+    opt.step()
+    for p, (w, m, v) in zip(ps, before):
+        m, g = m.double(), p.grad.double()
+        off = (opt.state[p]["exp_avg"].double() - (b1 * m + (1 - b1) * g)).abs()
+        bound = SPARE * U * (2 * b1 * m.abs() + 3 * (1 - b1) * g.abs()) + 2.0 ** -149
+        assert bool((off <= bound).all()), float((off / bound).max())
+
+
+def test_steps_of_both_betas_zero():
+    """betas (0, 0): whatever the moments were, the step is lr g / (|g| + eps).  With m = g exactly and v off by
+    U, the root by half of that, by U and by U of eps and the sum, and the division by U, the step is off by 4 U,
+    and the sum by U of the weight."""
+    ps, state = wide_case(torch.float32, 17)
+    hyper = dict(HYPER, betas=(0.0, 0.0), lr=0.25, eps=1e-5)
+    opt = make(ps, state, hyper)
+    before = snapshot(opt, ps, state)
+    opt.step()
+    for p, (w, m, v) in zip(ps, before):
+        g = p.grad.double()
+        step = 0.25 * g / (g.abs() + 1e-5)
+        want = w.double() - step
+        assert torch.equal(opt.state[p]["exp_avg"], p.grad)
+        off = (p.detach().double() - want).abs()
+        assert bool((off <= SPARE * U * (4 * step.abs() + want.abs())).all())

@@ -61,6 +61,7 @@ struct AdamArgs {
     double lr, log_beta1, log_beta2, weight_decay, max_norm;
     const float *lr_device;
     float rate1, rate2, eps;                 // 1 - b1, 1 - b2
+    float beta1;
     float decay;                             // in the gradient; 0 where it is decoupled
     int decoupled, maximize;
 };
@@ -364,12 +365,19 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(NormTable<NORM_TENSORS> 
 }
 
 // ---------------------------------------------------------------------------------- Adam
+// b1 m + (1 - b1) g.  Near 1 as m + (1 - b1)(g - m), since float32 holds 1 - b1 to 2^-24 of itself, b1
+// only to 2^-24 of 1; below 1/2 the roundings of m in g - m would count in full where m itself counts
+// with b1 (b1 = 0, m = 1, g = 1e-9: 0 instead of g).  One branch for the whole launch.
+__device__ inline float moment1(float m, float g, const AdamArgs &a) {
+    return a.rate1 > 0.5f ? fmaf(a.beta1, m, a.rate1 * g) : fmaf(a.rate1, g - m, m);
+}
+
 __device__ inline void adam_element(float &p, float g, float &m, float &v, const AdamArgs &a, const Rates &r, float c) {
     g *= c;
     g = a.maximize ? -g : g;
     if (a.decay != 0.0f) g = fmaf(a.decay, p, g);
     p *= r.keep;
-    m = fmaf(a.rate1, g - m, m);
+    m = moment1(m, g, a);
     // b2 v as v - (1 - b2) v: float32 holds 1 - b2 to 2^-24 of itself, b2 only to 2^-24 of 1, which
     // would move the average of a long run by 2^-24 / (1 - b2)
     const float kept = v < __builtin_inff() ? fmaf(-a.rate2, v, v) : v;
@@ -582,6 +590,7 @@ AdamArgs args_of(const cista_adam_group &q, double max_norm) {
     a.lr_device = q.lr_device;
     a.rate1 = (float)(1.0 - q.beta1);
     a.rate2 = (float)(1.0 - q.beta2);
+    a.beta1 = (float)q.beta1;
     a.eps = (float)q.eps;
     a.decay = q.decoupled ? 0.0f : (float)q.weight_decay;
     a.decoupled = q.decoupled;
