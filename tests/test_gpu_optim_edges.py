@@ -66,3 +66,20 @@ def test_steps_of_both_betas_zero():
         assert torch.equal(opt.state[p]["exp_avg"], p.grad)
         off = (p.detach().double() - want).abs()
         assert bool((off <= SPARE * U * (4 * step.abs() + want.abs())).all())
+
+
+@pytest.mark.parametrize("b2", [1e-9, 0.001, 0.1, 0.3, 0.49])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_second_moment_of_a_small_beta2(dtype, b2):
+    """As for the first: b2, its product with v and the sum are off by U each, and so are 1 - b2, its product with
+    g and the sum: 3 U of either term."""
+    ps, state = wide_case(dtype, 27)
+    opt = make(ps, state, dict(HYPER, betas=(0.9, b2)))
+    before = snapshot(opt, ps, state)
+    opt.step()
+    for p, (w, m, v) in zip(ps, before):
+        v, g = v.double(), p.grad.double()
+        want = b2 * v + (1 - b2) * g * g
+        off = (opt.state[p]["exp_avg_sq"].double() - want).abs()
+        bound = SPARE * 3 * U * want + 2.0 ** -149
+        assert bool((off <= bound).all()), float((off / bound).max())

@@ -61,7 +61,7 @@ struct AdamArgs {
     double lr, log_beta1, log_beta2, weight_decay, max_norm;
     const float *lr_device;
     float rate1, rate2, eps;                 // 1 - b1, 1 - b2
-    float beta1;
+    float beta1, beta2;
     float decay;                             // in the gradient; 0 where it is decoupled
     int decoupled, maximize;
 };
@@ -372,16 +372,21 @@ __device__ inline float moment1(float m, float g, const AdamArgs &a) {
     return a.rate1 > 0.5f ? fmaf(a.beta1, m, a.rate1 * g) : fmaf(a.rate1, g - m, m);
 }
 
+// b2 v + (1 - b2) g^2, with b2 v as v - (1 - b2) v: b2 itself, rounded, would move the average of a long
+// run by 2^-24 / (1 - b2).  Below 1/2 it is the other way round (b2 = 1e-9: 1 - b2 is 1, and nothing
+// of v would be left).
+__device__ inline float moment2(float v, float g, const AdamArgs &a) {
+    const float kept = a.rate2 > 0.5f ? a.beta2 * v : v < __builtin_inff() ? fmaf(-a.rate2, v, v) : v;
+    return fmaf(a.rate2 * g, g, kept);
+}
+
 __device__ inline void adam_element(float &p, float g, float &m, float &v, const AdamArgs &a, const Rates &r, float c) {
     g *= c;
     g = a.maximize ? -g : g;
     if (a.decay != 0.0f) g = fmaf(a.decay, p, g);
     p *= r.keep;
     m = moment1(m, g, a);
-    // b2 v as v - (1 - b2) v: float32 holds 1 - b2 to 2^-24 of itself, b2 only to 2^-24 of 1, which
-    // would move the average of a long run by 2^-24 / (1 - b2)
-    const float kept = v < __builtin_inff() ? fmaf(-a.rate2, v, v) : v;
-    v = fmaf(a.rate2 * g, g, kept);
+    v = moment2(v, g, a);
     p = fmaf(-r.size, m / fmaf(sqrtf(v), r.inv_root, a.eps), p);
 }
 
@@ -591,6 +596,7 @@ AdamArgs args_of(const cista_adam_group &q, double max_norm) {
     a.rate1 = (float)(1.0 - q.beta1);
     a.rate2 = (float)(1.0 - q.beta2);
     a.beta1 = (float)q.beta1;
+    a.beta2 = (float)q.beta2;
     a.eps = (float)q.eps;
     a.decay = q.decoupled ? 0.0f : (float)q.weight_decay;
     a.decoupled = q.decoupled;
