@@ -83,3 +83,38 @@ def test_second_moment_of_a_small_beta2(dtype, b2):
         off = (opt.state[p]["exp_avg_sq"].double() - want).abs()
         bound = SPARE * 3 * U * want + 2.0 ** -149
         assert bool((off <= bound).all()), float((off / bound).max())
+
+
+# ------------------------------------------------------------------------------------- one rounding
+def near_ties(dtype, seed):
+    """A scale c (float32) and values g of the type for which the float32 product, rounded to the type, differs from
+    the exact product rounded at once (for bfloat16, which no instruction rounds at once, any values)."""
+    r = np.random.default_rng(seed)
+    if dtype == torch.bfloat16:
+        return float(np.float32(r.uniform(0.5, 1.0))), torch.randn(4096, device=DEV, generator=gen(seed)).to(dtype)
+    g = np.arange(1024, 2048) * 2.0 ** -10                    # every significand of float16
+    for c in r.uniform(0.5, 1.0, 4000).astype(np.float32):
+        exact = g * float(c)                                  # 11 and 24 bits: exact in float64
+        hit = g[exact.astype(np.float16) != exact.astype(np.float32).astype(np.float16)]
+        if len(hit) >= 2:
+            return float(c), torch.tensor(np.concatenate([hit, -hit, 4 * hit]), device=DEV).to(dtype)
+    raise AssertionError("no such scale")
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_clipped_values_do_not_depend_on_their_place(dtype, seed):
+    """A 16-bit gradient is the float32 product rounded once, bit for bit, inside a tensor and at its ends."""
+    c, values = near_ties(dtype, seed)
+    sizes = [1, 3, 7, 8, 9, 15, 16, 33, 1, 1000, 4097, 8191, 30011]
+    total = sum(sizes) + 1
+    flat = values[torch.randint(len(values), (total,), device=DEV, generator=gen(seed))]
+    grads, at = [], 1
+    for n in sizes:
+        grads.append(flat[at:at + n])
+        at += n
+    want = [(g.float() * c).to(dtype) for g in grads]
+    norm = torch.tensor(2.0, device=DEV)
+    optim.clip_grads_with_norm_(params_of(grads), c * (2.0 + 1e-6), norm)
+    for g, w in zip(grads, want):
+        assert torch.equal(g, w), (g.numel(), int((g != w).sum()))

@@ -97,7 +97,8 @@ template <bool STREAM, typename T, int V> __device__ inline void store(T *p, con
 }
 
 // the 16-bit value of a float32 result as it is stored: an opaque register keeps the compiler from
-// rounding the last fma to 16 bits at once (v_fma_mixlo_f16), which is another value near a tie
+// rounding the last fma or product to 16 bits at once (v_fma_mixlo_f16), which is another value near
+// a tie, and which it does in some loops and not in others
 template <typename T> __device__ inline T rounded(float x) {
     asm("" : "+v"(x));
     return (T)x;
@@ -338,10 +339,10 @@ template <typename T> __device__ void scale_chunk(const Chunk<T> &k, float c) {
 #pragma unroll
     for (int u = 0; u < NORM_UNROLL; ++u) {
 #pragma unroll
-        for (int e = 0; e < k.V; ++e) x[u].e[e] = (T)(to_f32(x[u].e[e]) * c);
+        for (int e = 0; e < k.V; ++e) x[u].e[e] = rounded<T>(to_f32(x[u].e[e]) * c);
         if (k.full() || k.inside(u)) store<false>(k.base + k.at(u), x[u]);
     }
-    k.ends([&](GLOBAL T &g) { g = (T)(to_f32(g) * c); });
+    k.ends([&](GLOBAL T &g) { g = rounded<T>(to_f32(g) * c); });
 }
 
 // One block per chunk, each rounding once to the gradient's type, of a float32 product.  The chunks
