@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_optim import (DEV, HYPER, ODD, SPARE, TYPES, U, adam_bounds, adam_case, check_scaled, check_step, gen,  # noqa: F401
+from tests.test_gpu_optim import (DEV, HYPER, ODD, SPARE, TYPES, U, adam64, adam_case, check_scaled, check_step, gen,  # noqa: F401
                                   make, near, norm64, params_of, params_of_views, snapshot, some, way)
 from v2e2v_amd import _lib, optim
 
@@ -118,3 +118,82 @@ def test_clipped_values_do_not_depend_on_their_place(dtype, seed):
     optim.clip_grads_with_norm_(params_of(grads), c * (2.0 + 1e-6), norm)
     for g, w in zip(grads, want):
         assert torch.equal(g, w), (g.numel(), int((g != w).sum()))
+
+
+# ------------------------------------------------------------------------------------- small decay
+@pytest.mark.parametrize("lr,wd", [(1e-4, 0.01), (1e-5, 0.01), (2e-6, 0.01)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_small_decoupled_decay_over_many_steps(dtype, lr, wd):
+    """The mean weight of many after many steps.  Each step rounds a weight of [0.5, 1) by at most 2^-25, to either
+    side as the update's low bits fall (a deviation of 2^-24 / sqrt(12) each), so the mean of N weights is off by
+    2^-24 sqrt(K / (12 N)) in K steps: 8 of them, and 10 U of the updates' sum of magnitudes, are allowed.
+    lr wd rounded to multiples of 2^-24 instead is off by 1 % to 100 % of the decay."""
+    N, K = 200_000, 40
+    p = torch.nn.Parameter((0.6 + 0.3 * torch.rand(N, device=DEV, generator=gen(1))).to(dtype))
+    w = p.detach().double()
+    m = torch.randn(N, device=DEV, generator=gen(2)) * 0.3
+    v = 0.5 + torch.rand(N, device=DEV, generator=gen(3))
+    state = {0: dict(step=torch.tensor(1000.0), exp_avg=m.clone(), exp_avg_sq=v.clone(),
+                     **({} if dtype == torch.float32 else {"master": p.detach().float()}))}
+    b1, b2 = 0.9, 0.999
+    opt = make([p], state, dict(HYPER, lr=lr, weight_decay=wd, decoupled=True))
+    m, v, start, moved = m.double(), v.double(), w.mean().item(), 0.0
+    for k in range(K):
+        g = torch.randn(N, device=DEV, generator=gen(100 + k)).to(dtype)
+        p.grad = g
+        opt.step()
+        g, t = g.double(), 1001 + k
+        m = b1 * m + (1 - b1) * g
+        v = b2 * v + (1 - b2) * g * g
+        step = lr / (1 - b1 ** t) * m / ((v / (1 - b2 ** t)).sqrt() + 1e-8)
+        w = w * (1 - lr * wd) - step
+        moved += step.abs().mean().item()
+    got = opt.state[p]["master"] if dtype != torch.float32 else p.detach()
+    assert 0.5 < float(got.min()) and float(got.max()) < 1.0
+    off = abs(got.double().mean().item() - w.mean().item())
+    allowed = 8 * 2.0 ** -24 * math.sqrt(K / (12 * N)) + 10 * U * moved
+    assert allowed < 0.01 * K * lr * wd * start                        # what the bound can tell
+    assert off <= allowed, (off, allowed, K * lr * wd * start)
+
+
+@pytest.mark.parametrize("decay", [0.25, 0.49, 0.5, 0.75, 1.0])
+def test_large_decoupled_decay(decay):
+    """Where little of the old weight is left, its roundings count with what is left: decay is off by U (of 1 - decay
+    or of itself, below 1/2, where 1 - decay is at least as large), its product by U, the sum by U of the result, and
+    the update by 8 U."""
+    ps, state = wide_case(torch.float32, 37)
+    hyper = dict(HYPER, lr=1.0, weight_decay=decay, decoupled=True)
+    for s in state.values():
+        s["exp_avg"] *= 1e-6
+    opt = make(ps, state, hyper)
+    before = snapshot(opt, ps, state)
+    opt.step()
+    for p, (w, m, v) in zip(ps, before):
+        m1, v1 = opt.state[p]["exp_avg"].double(), opt.state[p]["exp_avg_sq"].double()
+        root = v1.sqrt() / math.sqrt(1 - 0.999 ** 4) + 1e-8
+        step = m1 / (1 - 0.9 ** 4) / root
+        want = w.double() * (1 - decay) - step
+        off = (p.detach().double() - want).abs()
+        # lr / (1 - b1^t), the division, the root, its factor and sum, the product and both sums: 8 U of the update
+        assert bool((off <= SPARE * U * (8 * step.abs() + 4 * (1 - decay) * w.double().abs()) + 2.0 ** -149).all())
+
+
+def test_decay_of_infinite_weights():
+    """p (1 - lr wd) of an infinity is that infinity; a NaN stays one, and their neighbours are the formula's."""
+    hyper = dict(HYPER, lr=1e-2, weight_decay=0.1, decoupled=True)
+    ps, state = adam_case([4099], torch.float32, 61, 3)
+    bad = torch.tensor([5, 1030, 4098], device=DEV)
+    with torch.no_grad():
+        ps[0][bad] = torch.tensor([math.inf, -math.inf, math.nan], device=DEV)
+    opt = make(ps, state, hyper)
+    before = snapshot(opt, ps, state)
+    opt.step()
+    got = ps[0].detach()[bad].tolist()
+    assert got[:2] == [math.inf, -math.inf] and math.isnan(got[2])
+    with torch.no_grad():
+        for w in (ps[0], before[0][0]):
+            w[bad] = 0.0
+        w1 = adam64(before[0][0], ps[0].grad, *before[0][1:], 4, 1.0, **hyper)
+        off = (ps[0].double() - w1[0]).abs()
+        off[bad] = 0.0
+        assert bool((off <= w1[3][0]).all())

@@ -52,9 +52,11 @@ template <int N> struct StepTable {
     float *step[N];
 };
 
-// what a tensor's update takes from its step count: lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
+// what a tensor's update takes from its step count: lr / (1 - b1^t), 1 / sqrt(1 - b2^t), and for
+// decoupled decay lr wd where that is below 1/2 (keep is 1), else 1 - lr wd (decay is 0): float32 holds
+// either to 2^-24 of itself, but 1 - lr wd near 1 only to multiples of 2^-24
 struct Rates {
-    float size, inv_root, keep, pad;
+    float size, inv_root, keep, decay;
 };
 
 struct AdamArgs {
@@ -129,8 +131,9 @@ __device__ inline void advance(float *step, const AdamArgs &a, Rates *rates) {
     Rates r;
     r.size = (float)(lr / -expm1((double)t * a.log_beta1));
     r.inv_root = (float)(1.0 / sqrt(-expm1((double)t * a.log_beta2)));
-    r.keep = a.decoupled ? (float)(1.0 - lr * a.weight_decay) : 1.0f;
-    r.pad = 0.0f;
+    const double decay = a.decoupled ? lr * a.weight_decay : 0.0;
+    r.keep = decay < 0.5 ? 1.0f : (float)(1.0 - decay);
+    r.decay = decay < 0.5 ? (float)decay : 0.0f;
     *rates = r;
 }
 
@@ -385,10 +388,14 @@ __device__ inline void adam_element(float &p, float g, float &m, float &v, const
     g *= c;
     g = a.maximize ? -g : g;
     if (a.decay != 0.0f) g = fmaf(a.decay, p, g);
-    p *= r.keep;
     m = moment1(m, g, a);
     v = moment2(v, g, a);
-    p = fmaf(-r.size, m / fmaf(sqrtf(v), r.inv_root, a.eps), p);
+    const float q = m / fmaf(sqrtf(v), r.inv_root, a.eps);
+    // decay and update leave the weight in one subtraction: a decay of less than half a step of float32
+    // would not move it by itself, and one rounded to whole steps would be off at every step alike.  An
+    // infinite weight, from which its own decay cannot be subtracted, goes the other way and stays.
+    const bool together = r.decay != 0.0f && fabsf(p) < __builtin_inff();
+    p = together ? p - fmaf(r.decay, p, r.size * q) : fmaf(-r.size, q, p * r.keep);
 }
 
 // Elements [chunk * ADAM_CHUNK - shift, + ADAM_CHUNK) of a tensor, 4 to a thread.  The shift puts the
