@@ -197,3 +197,33 @@ def test_decay_of_infinite_weights():
         off = (ps[0].double() - w1[0]).abs()
         off[bad] = 0.0
         assert bool((off <= w1[3][0]).all())
+
+
+# ------------------------------------------------------------------------------------- state
+def give_grads(ps, k):
+    for i, p in enumerate(ps):
+        p.grad = torch.randn(p.shape, device=DEV, generator=gen(10 * k + i)).to(p.dtype)
+
+
+@pytest.mark.parametrize("half", [torch.bfloat16, torch.float16])
+def test_a_phase_in_float32_is_not_undone(half):
+    """16-bit steps, float32 steps, 16-bit steps: the last ones go on from the float32 weights."""
+    net = torch.nn.Sequential(torch.nn.Linear(33, 40), torch.nn.Linear(40, 7)).to(DEV, half)
+    ps, hyper = list(net.parameters()), dict(HYPER, lr=0.1)
+    opt = make(ps, {}, hyper)
+    for t in range(2):
+        give_grads(ps, t)
+        opt.step()
+    net.float()
+    for t in range(2, 4):
+        give_grads(ps, t)
+        before = snapshot(opt, ps, {}) if t > 2 else None
+        opt.step()
+        assert all("master" not in opt.state[p] for p in ps)
+        if before:
+            check_step(opt, ps, before, hyper, t + 1, 1.0)
+    net.to(half)
+    give_grads(ps, 4)
+    before = [(p.detach().float(), opt.state[p]["exp_avg"].clone(), opt.state[p]["exp_avg_sq"].clone()) for p in ps]
+    opt.step()
+    check_step(opt, ps, before, hyper, 5, 1.0)

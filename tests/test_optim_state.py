@@ -1,0 +1,28 @@
+"""The optimizers' state (v2e2v_amd/optim.py) as it is loaded: what needs no GPU."""
+import pytest
+import torch
+
+from v2e2v_amd import optim
+
+
+def live(dtype, step=4.0):
+    """An optimizer of two parameters as it is in the middle of a run."""
+    ps = [torch.nn.Parameter(torch.ones(n, dtype=dtype)) for n in (3, 5)]
+    opt = optim.Adam(ps)
+    for p in ps:
+        opt.state[p] = dict(step=torch.tensor(step), exp_avg=torch.full_like(p, 0.25, dtype=torch.float32, requires_grad=False),
+                            exp_avg_sq=torch.full_like(p, 0.5, dtype=torch.float32, requires_grad=False))
+        if dtype != torch.float32:
+            opt.state[p]["master"] = p.detach().float() + 2.0 ** -12
+    return ps, opt
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_master_copy_goes_with_a_16_bit_parameter_only(dtype):
+    _, saved = live(torch.bfloat16)
+    ps, opt = live(dtype)
+    opt.load_state_dict(saved.state_dict())
+    for p in ps:
+        assert ("master" in opt.state[p]) == (dtype != torch.float32)
+        if dtype != torch.float32:
+            assert bool((opt.state[p]["master"] == 1 + 2.0 ** -12).all())

@@ -125,6 +125,12 @@ PyObject *item(PyObject *dict, PyObject *key) {
     return o;
 }
 
+bool has(PyObject *dict, PyObject *key) {
+    const int found = PyDict_Contains(dict, key);
+    if (found < 0) throw NotPlain();
+    return found;
+}
+
 double number(PyObject *o) {
     if (PyFloat_CheckExact(o)) return PyFloat_AS_DOUBLE(o);
     if (!PyLong_Check(o)) throw NotPlain();
@@ -224,6 +230,8 @@ PyObject *cista_torch_adam_step(PyObject *param_groups, PyObject *state, int nor
                 r.grad = r.numel ? grad.data_ptr() : nullptr;
                 r.exp_avg = moment(slot, key.exp_avg, p, device);
                 r.exp_avg_sq = moment(slot, key.exp_avg_sq, p, device);
+                // a float32 parameter has no master copy; one left from 16-bit steps is dropped in Python
+                if (r.type == CISTA_F32 && has(slot, key.master)) throw NotPlain();
                 r.master = r.type == CISTA_F32 ? nullptr : moment(slot, key.master, p, device);
                 r.step = step.data_ptr<float>();
                 rows.push_back(r);

@@ -231,8 +231,8 @@ class Adam(torch.optim.Optimizer):
     reads at each replay.  State of each parameter: ``step`` (float32 scalar on the device),
     ``exp_avg``, ``exp_avg_sq`` (float32, the parameter's shape) and, for a 16-bit parameter,
     ``master`` (float32; made from the parameter when first needed, so from then on a parameter
-    is changed through it).  A state_dict keeps those types when it is loaded; one without ``master``
-    loads too.  A captured step replays the update; weights that the network has packed are then
+    is changed through it; dropped by a step, or a state_dict loaded, while the parameter is float32).
+    A state_dict keeps those types when it is loaded; one without ``master`` loads too.  A captured step replays the update; weights that the network has packed are then
     repacked after ``model.invalidate_packed()``.
     """
 
@@ -283,7 +283,9 @@ class Adam(torch.optim.Optimizer):
             st["step"] = torch.full((), float(step), dtype=torch.float32, device=p.device)
         moment("exp_avg")
         moment("exp_avg_sq")
-        if p.dtype != torch.float32:
+        if p.dtype == torch.float32:
+            st.pop("master", None)                            # of 16-bit steps before: older than the parameter from here on
+        else:
             if st.get("master") is None:
                 made()
                 st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
@@ -311,6 +313,8 @@ class Adam(torch.optim.Optimizer):
                 t = state_dict["state"].get(i, {}).get(name)
                 if t is not None and p.dtype != torch.float32:
                     self.state[p][name] = t.to(device=p.device, dtype=torch.float32, copy=True)
+            if p.dtype == torch.float32 and p in self.state:
+                self.state[p].pop("master", None)
 
     def step(self, closure=None):
         loss = None
