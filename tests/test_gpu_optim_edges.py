@@ -227,3 +227,23 @@ def test_a_phase_in_float32_is_not_undone(half):
     before = [(p.detach().float(), opt.state[p]["exp_avg"].clone(), opt.state[p]["exp_avg_sq"].clone()) for p in ps]
     opt.step()
     check_step(opt, ps, before, hyper, 5, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_state_loaded_from_a_live_optimizer(dtype):
+    """Two optimizers that go on from one state: neither moves the other's moments or step counts."""
+    ps, _ = adam_case([5, 3000], dtype, 12, 0)
+    a = optim.Adam(ps, lr=0.1)
+    a.step()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    for p, q in zip(ps, qs):
+        q.grad = p.grad.clone()
+    b = optim.Adam(qs, lr=0.1)
+    b.load_state_dict(a.state_dict())
+    kept = {n: [a.state[p][n].clone() for p in ps] for n in a.state[ps[0]]}
+    b.step()
+    assert all(torch.equal(a.state[p][n], old) for n in kept for p, old in zip(ps, kept[n]))
+    a.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q) and a.state[p]["step"].item() == b.state[q]["step"].item() == 2
+        assert all(torch.equal(a.state[p][n], b.state[q][n]) for n in kept)

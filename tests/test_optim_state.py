@@ -26,3 +26,18 @@ def test_a_master_copy_goes_with_a_16_bit_parameter_only(dtype):
         assert ("master" in opt.state[p]) == (dtype != torch.float32)
         if dtype != torch.float32:
             assert bool((opt.state[p]["master"] == 1 + 2.0 ** -12).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_loaded_state_is_a_copy(dtype):
+    """The state_dict of a live optimizer: neither one's step counts or moments are the other's memory."""
+    ps, saved = live(dtype)
+    qs, opt = live(dtype, 9.0)
+    opt.load_state_dict(saved.state_dict())
+    for p, q in zip(ps, qs):
+        assert set(opt.state[q]) == set(saved.state[p])
+        for name, t in opt.state[q].items():
+            assert torch.equal(t, saved.state[p][name]) and t.data_ptr() != saved.state[p][name].data_ptr(), name
+    a = optim.Adam([torch.nn.Parameter(torch.ones(2))])
+    a.load_state_dict(dict(state={0: dict(step=3)}, param_groups=a.state_dict()["param_groups"]))    # a plain number
+    assert a.state[a.param_groups[0]["params"][0]]["step"] == 3

@@ -304,7 +304,8 @@ class Adam(torch.optim.Optimizer):
                 g.setdefault(k, v)
 
     def load_state_dict(self, state_dict):
-        """The state keeps its float32 values (the base class casts it to the parameter's type)."""
+        """The state keeps its float32 values (the base class casts it to the parameter's type), in memory of
+        its own: step counts and moments are advanced in place, and the state_dict may be a live optimizer's."""
         super().load_state_dict(state_dict)
         params = [p for g in self.param_groups for p in g["params"]]
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -313,8 +314,13 @@ class Adam(torch.optim.Optimizer):
                 t = state_dict["state"].get(i, {}).get(name)
                 if t is not None and p.dtype != torch.float32:
                     self.state[p][name] = t.to(device=p.device, dtype=torch.float32, copy=True)
-            if p.dtype == torch.float32 and p in self.state:
+            if p not in self.state:
+                continue
+            if p.dtype == torch.float32:
                 self.state[p].pop("master", None)
+            for name, t in self.state[p].items():             # what the base class took over as it is
+                if isinstance(t, torch.Tensor) and t is state_dict["state"].get(i, {}).get(name):
+                    self.state[p][name] = t.clone()
 
     def step(self, closure=None):
         loss = None
