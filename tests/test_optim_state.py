@@ -41,3 +41,25 @@ def test_a_loaded_state_is_a_copy(dtype):
     a = optim.Adam([torch.nn.Parameter(torch.ones(2))])
     a.load_state_dict(dict(state={0: dict(step=3)}, param_groups=a.state_dict()["param_groups"]))    # a plain number
     assert a.state[a.param_groups[0]["params"][0]]["step"] == 3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_hooks_of_load_state_dict(dtype):
+    """What a pre-hook returns is what is loaded, and a post-hook sees the state that stays."""
+    _, saved = live(dtype)
+    qs, opt = live(dtype, 9.0)
+    value = 0.125 + 2.0 ** -20                               # no 16-bit value
+    seen = []
+
+    def doubled(o, sd):
+        return dict(sd, state={i: dict(s, exp_avg=torch.full_like(s["exp_avg"], value)) for i, s in sd["state"].items()})
+
+    opt.register_load_state_dict_pre_hook(doubled)
+    opt.register_load_state_dict_post_hook(lambda o: seen.extend(o.state[q]["exp_avg"] for q in qs))
+    for _ in range(2):
+        opt.load_state_dict(saved.state_dict())
+        assert len(seen) == 2
+        for q, t in zip(qs, seen):
+            assert opt.state[q]["exp_avg"] is t and t.dtype == torch.float32 and bool((t == value).all())
+        seen.clear()
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 1

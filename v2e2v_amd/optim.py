@@ -305,22 +305,31 @@ class Adam(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """The state keeps its float32 values (the base class casts it to the parameter's type), in memory of
-        its own: step counts and moments are advanced in place, and the state_dict may be a live optimizer's."""
-        super().load_state_dict(state_dict)
+        its own: step counts and moments are advanced in place, and the state_dict may be a live optimizer's.
+        What is loaded is what pre-hooks make of the state_dict; post-hooks see the state as it stays."""
+        loaded = []
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, d: loaded.append(d)),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_over(loaded[-1]), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    def _take_over(self, state_dict):
         params = [p for g in self.param_groups for p in g["params"]]
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, params):
-            for name in ("exp_avg", "exp_avg_sq", "master"):
-                t = state_dict["state"].get(i, {}).get(name)
-                if t is not None and p.dtype != torch.float32:
-                    self.state[p][name] = t.to(device=p.device, dtype=torch.float32, copy=True)
             if p not in self.state:
                 continue
+            given, mine = state_dict["state"].get(i, {}), self.state[p]
+            for name, t in mine.items():
+                if name in ("exp_avg", "exp_avg_sq", "master") and p.dtype != torch.float32 and given.get(name) is not None:
+                    mine[name] = given[name].to(device=p.device, dtype=torch.float32, copy=True)
+                elif isinstance(t, torch.Tensor) and t is given.get(name):      # taken over as it is
+                    mine[name] = t.clone()
             if p.dtype == torch.float32:
-                self.state[p].pop("master", None)
-            for name, t in self.state[p].items():             # what the base class took over as it is
-                if isinstance(t, torch.Tensor) and t is state_dict["state"].get(i, {}).get(name):
-                    self.state[p][name] = t.clone()
+                mine.pop("master", None)
 
     def step(self, closure=None):
         loss = None
