@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from v2e2v_amd import optim
+from v2e2v_amd import _lib, optim
 
 
 def live(dtype, step=4.0):
@@ -63,3 +63,16 @@ def test_hooks_of_load_state_dict(dtype):
             assert opt.state[q]["exp_avg"] is t and t.dtype == torch.float32 and bool((t == value).all())
         seen.clear()
     assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 1
+
+
+def test_a_refused_state_dict_changes_nothing():
+    """amsgrad is refused before the state or the hyperparameters are taken over."""
+    _, saved = live(torch.float32)
+    qs, opt = live(torch.float32, 9.0)
+    sd = saved.state_dict()
+    sd["param_groups"][0].update(amsgrad=True, lr=123.0)
+    with pytest.raises(_lib.CistaError, match="amsgrad"):
+        opt.load_state_dict(sd)
+    assert "amsgrad" not in opt.param_groups[0] and opt.param_groups[0]["lr"] == 1e-3
+    assert all(opt.state[q]["step"].item() == 9.0 for q in qs)
+    assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks

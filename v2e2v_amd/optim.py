@@ -295,11 +295,15 @@ class Adam(torch.optim.Optimizer):
     def __getstate__(self):
         return dict(super().__getstate__(), max_norm=self.max_norm, norm_type=self.norm_type, grad_norm=None)
 
+    @staticmethod
+    def _refuse_amsgrad(state):
+        if any(g.get("amsgrad") for g in state["param_groups"]):
+            raise _lib.CistaError("amsgrad is not built")
+
     def __setstate__(self, state):
+        self._refuse_amsgrad(state)                           # before anything is taken over
         super().__setstate__(state)
         for g in self.param_groups:
-            if g.get("amsgrad"):
-                raise _lib.CistaError("amsgrad is not built")
             for k, v in self.defaults.items():
                 g.setdefault(k, v)
 
@@ -308,7 +312,12 @@ class Adam(torch.optim.Optimizer):
         its own: step counts and moments are advanced in place, and the state_dict may be a live optimizer's.
         What is loaded is what pre-hooks make of the state_dict; post-hooks see the state as it stays."""
         loaded = []
-        hooks = [self.register_load_state_dict_pre_hook(lambda _, d: loaded.append(d)),
+
+        def last(_, given):
+            self._refuse_amsgrad(given)
+            loaded.append(given)
+
+        hooks = [self.register_load_state_dict_pre_hook(last),
                  self.register_load_state_dict_post_hook(lambda _: self._take_over(loaded[-1]), prepend=True)]
         try:
             super().load_state_dict(state_dict)
