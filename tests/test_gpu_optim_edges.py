@@ -247,3 +247,47 @@ def test_state_loaded_from_a_live_optimizer(dtype):
     for p, q in zip(ps, qs):
         assert torch.equal(p, q) and a.state[p]["step"].item() == b.state[q]["step"].item() == 2
         assert all(torch.equal(a.state[p][n], b.state[q][n]) for n in kept)
+
+
+# ------------------------------------------------------------------------------------- views
+def overlapping():
+    base = torch.randn(12, 20, device=DEV, generator=gen(9))
+    z = torch.complex(base[0], base[1])
+    yield "the same strided view twice", base, [base[::2, ::3], base[::2, ::3]]
+    yield "a strided and a dense one", base, [base[:, 1:5:2], base[4]]
+    yield "a dense and a strided one, far apart in the list", base, [base[4, :3], torch.ones(3, device=DEV), base[3:, 2::7]]
+    yield "one element in common", base, [base[:6, :11:5], base[5:, 10::9]]
+    yield "a view and its transposed one", base, [base[:5, :5], base[:5, :5].t()]
+    yield "a negated view and its base", torch.view_as_real(z), [torch.view_as_real(z)[:, 1], z.conj().imag]
+    yield "an overlap with itself beside another", base, [base.reshape(-1).as_strided((4, 4), (2, 3)), base.reshape(-1)[15:16]]
+
+
+@pytest.mark.parametrize("k", range(7))
+def test_strided_gradients_that_share_memory_are_refused(k):
+    name, base, grads = list(overlapping())[k]
+    kept = base.clone()
+    version = [g._version for g in grads]
+    for call in (lambda: optim.clip_grad_norm_(params_of_views(grads), 1e-3),
+                 lambda: optim.clip_grads_with_norm_(params_of_views(grads), 1e-3, torch.tensor(1.0, device=DEV)),
+                 lambda: optim.clip_grad_norm_(params_of_views(grads), 1e-3, error_if_nonfinite=True)):
+        with pytest.raises(_lib.CistaError, match="overlap"):
+            call()
+        assert torch.equal(base, kept), name
+    assert [g._version for g in grads] == version
+    near(optim.grad_norm(grads), norm64(grads, 2), 2)                    # reading them is allowed
+
+
+def test_views_that_lie_between_each_other_are_clipped():
+    """Columns, halves of rows, real and imaginary parts, every second element: disjoint, in one buffer."""
+    base = torch.randn(16, 30, device=DEV, generator=gen(19))
+    z = torch.complex(base[0], base[1])
+    flat = base.reshape(-1)
+    for grads in ([base[:, k] for k in range(30)], [base[:, :7], base[:, 7:]], [z.real, z.imag], [z.real, z.conj().imag],
+                  [flat[::2], flat[1::2]], [base[::2, ::2], base[1::2].t(), base[::2, 1::2]], [base[:0, ::2], base[:, ::2]]):
+        for limit in (0.5, 0.125):                                       # the first one scales the buffer once only
+            old = [g.clone() for g in grads]
+            norm = norm64(old, 2)
+            near(optim.clip_grad_norm_(params_of_views(grads), limit), norm, 2)
+            check_scaled([g.clone() for g in grads], old, min(1.0, limit / (norm + 1e-6)))
+            with torch.no_grad():
+                base.mul_(8.0)

@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import math
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -154,8 +155,35 @@ def grad_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
     return norm
 
 
+class _Memory:
+    """A tensor's elements as numpy describes an array's; their memory is never touched."""
+
+    def __init__(self, t):
+        size, at = t.element_size(), t.data_ptr()
+        self.dense, self.begin, self.end = _dense(t), at, at
+        if t.numel():
+            self.end += size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+        self.__array_interface__ = dict(version=3, data=(at, False), typestr=f"|V{size}", shape=tuple(t.shape),
+                                        strides=tuple(s * size for s in t.stride()))
+
+
+def _refuse_shared(grads):
+    """Raises if an element of one gradient is another's too, where a copy would stand for one of them (the
+    library checks the others).  Views may lie between each other: columns of a matrix, real and imaginary parts."""
+    if all(_dense(g) for g in grads):
+        return
+    open_ = []                                               # those that reach past the next one's begin
+    for m in sorted((_Memory(g) for g in grads if g.numel()), key=lambda m: m.begin):
+        open_ = [o for o in open_ if o.end > m.begin]
+        for o in open_:
+            if not (o.dense and m.dense) and np.shares_memory(np.asarray(o), np.asarray(m)):
+                raise _lib.CistaError("a gradient overlaps another one: those that share memory cannot be written")
+        open_.append(m)
+
+
 def _written(grads, call):
     """Runs `call` on dense stand-ins of the gradients, and writes those that are copies back."""
+    _refuse_shared(grads)
     torch.autograd.graph.increment_version(grads)        # raises for what may not be written
     dense = [g if _dense(g) else g.resolve_neg().contiguous() for g in grads]
     call(dense)
