@@ -291,3 +291,28 @@ def test_views_that_lie_between_each_other_are_clipped():
             check_scaled([g.clone() for g in grads], old, min(1.0, limit / (norm + 1e-6)))
             with torch.no_grad():
                 base.mul_(8.0)
+
+
+def negated(t):
+    """The same values, as a lazily negated view of their opposites."""
+    return t.neg()._neg_view()
+
+
+def test_negated_views_count_with_their_sign():
+    """As the given norm, the learning rate, and the optimizer's state."""
+    grads = some([5, 4097], torch.float32, 3)
+    old = [g.clone() for g in grads]
+    total = negated(torch.tensor(4.0, device=DEV))
+    assert total.is_neg() and total.item() == 4.0
+    optim.clip_grads_with_norm_(params_of(grads), 1.0, total)
+    check_scaled(grads, old, 1.0 / (4.0 + 1e-6))
+    for dtype in (torch.float32, torch.bfloat16):
+        hyper = dict(HYPER, lr=0.25)
+        ps, state = adam_case([5, 3000], dtype, 81, 3)
+        opt = make(ps, state, hyper)
+        opt.param_groups[0]["lr"] = negated(torch.tensor(0.25, device=DEV))
+        for p in ps:
+            opt.state[p].update({n: negated(t.to(DEV)) for n, t in opt.state[p].items()})
+        before = snapshot(opt, ps, {})
+        opt.step()
+        check_step(opt, ps, before, hyper, 4, 1.0)

@@ -212,7 +212,7 @@ def clip_grads_with_norm_(parameters, max_norm, total_norm):
     if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1 or total_norm.device != dev:
         raise _lib.CistaError(f"total_norm must be a scalar tensor on {dev}")
     with _on(dev), torch.no_grad():
-        total = total_norm.detach().to(torch.float32)
+        total = total_norm.detach().to(torch.float32).resolve_neg()
         _written(grads, lambda dense: _lib.check(
             _lib.lib().cista_scale_grads(_table(dense), len(dense), max_norm, total.data_ptr(), _lib.stream_handle(dev)),
             "cista_scale_grads"))
@@ -298,7 +298,8 @@ class Adam(torch.optim.Optimizer):
             if t is None:
                 made()
                 t = torch.zeros_like(p, dtype=torch.float32, requires_grad=False)
-            elif t.dtype != torch.float32 or t.device != p.device or t.shape != p.shape or t.stride() != p.stride():
+            elif (t.dtype != torch.float32 or t.device != p.device or t.shape != p.shape or t.stride() != p.stride()
+                  or t.is_neg()):
                 if t.shape != p.shape:
                     raise _lib.CistaError(f"state {name} has shape {tuple(t.shape)}, its parameter {tuple(p.shape)}")
                 made()
@@ -306,7 +307,7 @@ class Adam(torch.optim.Optimizer):
             st[name] = t
 
         step = st.get("step", 0.0)
-        if not isinstance(step, torch.Tensor) or step.dtype != torch.float32 or step.device != p.device:
+        if not isinstance(step, torch.Tensor) or step.dtype != torch.float32 or step.device != p.device or step.is_neg():
             made()
             st["step"] = torch.full((), float(step), dtype=torch.float32, device=p.device)
         moment("exp_avg")
@@ -410,7 +411,8 @@ class Adam(torch.optim.Optimizer):
                 if lr.is_cuda:
                     if lr.dtype != torch.float32 or (params and lr.device != params[0].device):
                         raise _lib.CistaError("lr as a tensor must be float32, on the parameters' device")
-                    lr, lr_device = 0.0, lr.data_ptr()
+                    keep.append(lr.resolve_neg())
+                    lr, lr_device = 0.0, keep[-1].data_ptr()
                 else:
                     lr = float(lr)
             groups.append((lr, g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], lr_device, len(params),
