@@ -316,3 +316,19 @@ def test_negated_views_count_with_their_sign():
         before = snapshot(opt, ps, {})
         opt.step()
         check_step(opt, ps, before, hyper, 4, 1.0)
+
+
+def test_scalars_of_other_sizes_are_refused():
+    p = torch.nn.Parameter(torch.ones(3, device=DEV))
+    p.grad = torch.ones(3, device=DEV)
+    opt = optim.Adam([p])
+    for n in (0, 2):
+        opt.state[p]["step"] = torch.zeros(n, device=DEV)
+        with pytest.raises(_lib.CistaError, match="state step"):
+            opt.step()
+    del opt.state[p]["step"]
+    for n in (0, 2):
+        opt.param_groups[0]["lr"] = torch.ones(n, device=DEV)
+        with pytest.raises(_lib.CistaError, match="lr as a tensor"):
+            opt.step()
+    assert torch.equal(p.detach(), torch.ones(3, device=DEV))

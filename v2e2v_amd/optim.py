@@ -307,6 +307,8 @@ class Adam(torch.optim.Optimizer):
             st[name] = t
 
         step = st.get("step", 0.0)
+        if isinstance(step, torch.Tensor) and step.numel() != 1:
+            raise _lib.CistaError(f"state step has {step.numel()} elements")
         if not isinstance(step, torch.Tensor) or step.dtype != torch.float32 or step.device != p.device or step.is_neg():
             made()
             st["step"] = torch.full((), float(step), dtype=torch.float32, device=p.device)
@@ -409,8 +411,8 @@ class Adam(torch.optim.Optimizer):
             lr, lr_device = g["lr"], None
             if isinstance(lr, torch.Tensor):
                 if lr.is_cuda:
-                    if lr.dtype != torch.float32 or (params and lr.device != params[0].device):
-                        raise _lib.CistaError("lr as a tensor must be float32, on the parameters' device")
+                    if lr.dtype != torch.float32 or lr.numel() != 1 or (params and lr.device != params[0].device):
+                        raise _lib.CistaError("lr as a tensor must be one float32, on the parameters' device")
                     keep.append(lr.resolve_neg())
                     lr, lr_device = 0.0, keep[-1].data_ptr()
                 else:
