@@ -46,11 +46,11 @@ size_t cista_optim_workspace_bytes(int n);
 int cista_grad_norm(const cista_tensor *grads, int n, int norm_kind, float *norm, void *workspace,
                     size_t workspace_bytes, void *stream);
 
-/* grads <- c grads with a norm that is given (float32, device).  The tensors are disjoint
- * (checked: CISTA_ERR_ALIAS). */
+/* grads <- c grads with a norm that is given (float32, device).  The tensors are disjoint, and the
+ * norm is outside them (checked: CISTA_ERR_ALIAS). */
 int cista_scale_grads(const cista_tensor *grads, int n, double max_norm, const float *norm, void *stream);
 
-/* both: *norm = the norm before clipping, grads <- c grads */
+/* both: *norm = the norm before clipping, grads <- c grads; the same holds of the tensors and the norm */
 int cista_clip_grads(const cista_tensor *grads, int n, int norm_kind, double max_norm, float *norm, void *workspace,
                      size_t workspace_bytes, void *stream);
 
@@ -77,8 +77,9 @@ typedef struct {
 /* One step over all groups; the table holds the groups' tensors one group after the other.
  * norm_kind 0: no clipping (max_norm and norm are not used); else every gradient is scaled by c
  * of the norm over all groups, which goes to *norm; the gradients in memory stay as they are.
- * The parameters are disjoint, and so are the m, the v, the master copies and the steps (checked:
- * CISTA_ERR_ALIAS). */
+ * The parameters are disjoint, and so are the m, the v, the master copies and the steps, and the
+ * norm is outside them and the gradients (checked: CISTA_ERR_ALIAS); nor do two of these kinds share
+ * memory (not checked). */
 int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *groups, int n_groups, int norm_kind,
                     double max_norm, float *norm, void *workspace, size_t workspace_bytes, void *stream);
 

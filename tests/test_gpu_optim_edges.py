@@ -332,3 +332,11 @@ def test_scalars_of_other_sizes_are_refused():
         with pytest.raises(_lib.CistaError, match="lr as a tensor"):
             opt.step()
     assert torch.equal(p.detach(), torch.ones(3, device=DEV))
+
+
+def test_a_norm_that_is_a_gradient_is_refused():
+    grads = some([5, 4097], torch.float32, 3)
+    old = [g.clone() for g in grads]
+    with pytest.raises(_lib.CistaError, match="overlaps"):
+        optim.clip_grads_with_norm_(params_of(grads), 1e-3, grads[1][7])
+    assert all(torch.equal(a, b) for a, b in zip(grads, old))

@@ -186,3 +186,20 @@ def test_bench_flags(monkeypatch):
         monkeypatch.setattr(sys, "argv", ["bench.py"] + argv)
         with pytest.raises(SystemExit):
             bench.parse()
+
+
+@pytest.mark.parametrize("norm", [FAKE, FAKE + 32, FAKE + 60, FAKE * 8 + 8])
+def test_a_norm_within_the_tensors_is_refused(norm):
+    """Some workgroups would read, or write, it while others write the tensor."""
+    L = _lib.lib()
+    t = table((FAKE, 16, 0), (FAKE * 8, 3, 0))
+    assert L.cista_scale_grads(t, 2, 1.0, norm, None) == 5
+    assert L.cista_clip_grads(t, 2, 2, 1.0, norm, FAKE * 16, 1 << 30, None) == 5
+
+
+@pytest.mark.parametrize("k", [0, 1, 2, 3, 4, 5])
+def test_a_norm_within_the_state_is_refused(k):
+    row = adam_row(master=6 * FAKE, kind=1)
+    at = row[k] + (0 if k == 5 else 4)
+    assert adam_call([adam_row(9 * FAKE, 10 * FAKE, 11 * FAKE, 12 * FAKE, step=13 * FAKE), row], norm_kind=2, max_norm=1.0,
+                     norm=at, ws=16 * FAKE) == 5

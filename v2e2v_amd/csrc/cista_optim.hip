@@ -513,6 +513,24 @@ Range range_of(const void *data, long long numel, long long type) {
     return {(uintptr_t)data, (uintptr_t)data + (uintptr_t)numel * size_of(type)};
 }
 
+// is the float x within the tensor?  A norm is read, or written, by some workgroups while others write theirs
+bool holds(const float *x, const void *data, long long numel, long long type) {
+    const Range r = range_of(data, numel, type);
+    return (uintptr_t)x < r.end && (uintptr_t)x + sizeof(float) > r.begin;
+}
+
+bool holds(const float *x, const cista_tensor *t, int n) {
+    for (int i = 0; i < n; ++i)
+        if (holds(x, t[i].data, t[i].numel, t[i].type)) return true;
+    return false;
+}
+
+bool holds(const float *x, const cista_adam_tensor &t) {
+    return holds(x, t.param, t.numel, t.type) || holds(x, t.grad, t.numel, t.type) ||
+           holds(x, t.exp_avg, t.numel, CISTA_F32) || holds(x, t.exp_avg_sq, t.numel, CISTA_F32) ||
+           (t.type != CISTA_F32 && holds(x, t.master, t.numel, CISTA_F32)) || holds(x, t.step, 1, CISTA_F32);
+}
+
 int check(const cista_tensor *t, int n, bool written) {
     if (n < 0 || (n && !t)) return CISTA_ERR_INVALID;
     long long total = 0;
@@ -655,6 +673,7 @@ int cista_scale_grads(const cista_tensor *grads, int n, double max_norm, const f
     const int st = check(grads, n, true);
     if (st != CISTA_OK) return st;
     if (!norm || misplaced(norm) || !(max_norm >= 0.0)) return CISTA_ERR_INVALID;
+    if (holds(norm, grads, n)) return CISTA_ERR_ALIAS;
     return scale(grads, n, max_norm, {norm, nullptr, nullptr, 0, 0}, (hipStream_t)stream);
 }
 
@@ -666,6 +685,7 @@ int cista_clip_grads(const cista_tensor *grads, int n, int norm_kind, double max
         misplaced(norm) || misplaced(workspace))
         return CISTA_ERR_INVALID;
     if (workspace_bytes < cista_optim_workspace_bytes(n)) return CISTA_ERR_WORKSPACE;
+    if (holds(norm, grads, n)) return CISTA_ERR_ALIAS;
     hipStream_t s = (hipStream_t)stream;
     NormSource q = partials_of(norm_kind, false, n, [&](int i) { return grads[i]; }, norm, (double *)workspace, s);
     // without partial values (nothing but empty tensors) no other launch would write the norm
@@ -694,6 +714,7 @@ int cista_adam_step(const cista_adam_tensor *table, const cista_adam_group *grou
             (x.type != CISTA_F32 && bad_tensor(x.master, x.numel, CISTA_F32)))
             return CISTA_ERR_INVALID;
         if (x.numel > MOST_ADAM || (total += x.numel) > MOST_ADAM) return CISTA_ERR_UNSUPPORTED;
+        if (norm_kind && holds(norm, x)) return CISTA_ERR_ALIAS;
     }
     int apart = overlap(n, [&](int i) { return range_of(table[i].param, table[i].numel, table[i].type); });
     for (auto which : {&cista_adam_tensor::exp_avg, &cista_adam_tensor::exp_avg_sq, &cista_adam_tensor::master,
