@@ -1,0 +1,65 @@
+"""Which parameters' versions a step of torch's fused optimizers advances: those of every CistaLSTCNet in the
+stepped memory, however the network was made, and no other model's."""
+import copy
+import gc
+import pickle
+import weakref
+
+import pytest
+import torch
+
+from v2e2v_amd import CistaLSTCNet
+
+
+def small():
+    return CistaLSTCNet([16, 16], base_channels=32, depth=2, num_bins=5)
+
+
+def with_grads(params):
+    for p in params:
+        p.grad = torch.ones_like(p)
+    return params
+
+
+def test_other_models_are_left_alone():
+    """A fused step between another model's forward and its backward stays possible beside a network."""
+    net = small()
+    other = torch.nn.Sequential(torch.nn.Linear(3, 4), torch.nn.Linear(4, 2))
+    params = with_grads(list(other.parameters()))
+    opt = torch.optim.SGD(params, lr=0.1, fused=True)
+    before = [p._version for p in params]
+    out = other(torch.ones(5, 3)).sum()
+    opt.step()
+    assert [p._version for p in params] == before
+    out.backward()
+    del net
+
+
+@pytest.mark.parametrize("made", ["deepcopy", "pickle", "part", "flat"])
+def test_every_network_is_seen(made):
+    """A copy, an unpickled network, one inside another module, and one whose parameters are views of a flat
+    tensor that is stepped as a whole."""
+    net = small()
+    if made == "deepcopy":
+        net = copy.deepcopy(net)
+    elif made == "pickle":
+        net = pickle.loads(pickle.dumps(net))
+    stepped = list((torch.nn.ModuleDict(dict(a=net, b=torch.nn.Linear(2, 2))) if made == "part" else net).parameters())
+    if made == "flat":
+        flat = torch.nn.Parameter(torch.cat([p.detach().reshape(-1) for p in stepped]))
+        at = 0
+        for p in stepped:
+            p.data = flat.detach()[at:at + p.numel()].view(p.shape)
+            at += p.numel()
+        stepped = [flat]
+    params = list(net.parameters())
+    opt = torch.optim.Adam(with_grads(stepped), lr=0.1, fused=True)
+    before = [p._version for p in params]
+    opt.step()
+    assert all(p._version > v for p, v in zip(params, before))
+
+
+def test_networks_are_not_kept_alive():
+    ref = weakref.ref(small())
+    gc.collect()
+    assert ref() is None

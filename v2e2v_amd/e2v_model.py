@@ -35,19 +35,33 @@ from . import _lib
 from .base_layers import ConvLayer, ConvLSTC, IstaBlock, RecurrentConvLayer, UpsampleConvLayer
 
 
+_networks = weakref.WeakSet()                 # every CistaLSTCNet there is
+
+
+def _memory(p):
+    return p.untyped_storage()._cdata if p.layout == torch.strided else id(p)
+
+
 def _versions_after_fused_step(optimizer, args, kwargs):
     """torch's ``fused=True`` optimizers write the parameters without advancing the versions that
     packed_params and _grad_conduit go by: a network trained with one kept its first packed
-    weights.  This runs after every optimizer step and advances them."""
-    for g in optimizer.param_groups:
-        if g.get("fused"):
-            torch.autograd.graph.increment_version([p for p in g["params"] if p.grad is not None])
+    weights.  This runs after every optimizer step and advances those of the networks' parameters in
+    the memory that was stepped (they may be views of a flat one); other models' stay as they are."""
+    stepped = {_memory(p) for g in optimizer.param_groups if g.get("fused") for p in g["params"] if p.grad is not None}
+    if stepped:
+        own = [p for net in list(_networks) if "_parameters" in net.__dict__ for p in net.parameters()]
+        torch.autograd.graph.increment_version([p for p in own if _memory(p) in stepped])
 
 
 register_optimizer_step_post_hook(_versions_after_fused_step)
 
 
 class CistaLSTCNet(nn.Module):
+    def __new__(cls, *args, **kwargs):        # copies and unpickled networks come through here too
+        net = super().__new__(cls)
+        _networks.add(net)
+        return net
+
     def __init__(self, image_dim, base_channels=64, depth=5, num_bins=5):
         super().__init__()
         self.num_bins = num_bins
