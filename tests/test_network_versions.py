@@ -63,3 +63,20 @@ def test_networks_are_not_kept_alive():
     ref = weakref.ref(small())
     gc.collect()
     assert ref() is None
+
+
+@pytest.mark.parametrize("closure", [False, True])
+def test_gradients_cleared_by_a_hook_of_the_step(closure):
+    """The optimizer's own post-hook runs before anything global: the parameters were stepped all the same."""
+    net = small()
+    params = list(net.parameters())
+    opt = torch.optim.Adam(params if closure else with_grads(params), lr=0.1, fused=True)
+    opt.register_step_post_hook(lambda o, args, kwargs: o.zero_grad())
+
+    def loss():
+        with_grads(params)
+        return torch.tensor(1.0)
+
+    before = [(p._version, p.detach().clone()) for p in params]
+    opt.step(loss if closure else None)
+    assert all(p.grad is None and p._version > v and not torch.equal(p.detach(), old) for p, (v, old) in zip(params, before))
