@@ -12,7 +12,7 @@ OBJ  = build/cista_abi.o build/cista_voxel.o build/cista_ssim.o build/cista_v2e.
 # host library between Python's lists of tensors and the C ABI (links the installed torch)
 TLIB  = v2e2v_amd/libcista_torch.so
 PY    ?= python3
-TORCH = $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(u.find_spec('torch').origin))")
+TORCH := $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(u.find_spec('torch').origin))")
 PYINC = $(shell $(PY) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
 
 all: $(LIB) $(TLIB)
@@ -43,7 +43,8 @@ build/cista_optim.o: v2e2v_amd/csrc/cista_optim.hip include/cista_optim.h includ
 $(LIB): $(OBJ)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -o $@ $(OBJ)
 
-$(TLIB): v2e2v_amd/csrc/cista_torch.cpp include/cista_optim.h include/cista_lstc.h
+# version.py: another torch has another C++ ABI (_lib.torch_lib() refuses a library built for one)
+$(TLIB): v2e2v_amd/csrc/cista_torch.cpp include/cista_optim.h include/cista_lstc.h $(TORCH)/version.py Makefile
 	$(CXX) -O2 -std=c++17 -fPIC -Wall -shared -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -I$(PYINC) -isystem $(TORCH)/include \
 	    -isystem $(TORCH)/include/torch/csrc/api/include -isystem /opt/rocm/include -o $@ $< \
 	    -L$(TORCH)/lib -ltorch_python -ltorch_cpu -lc10 -lc10_hip

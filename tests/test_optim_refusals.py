@@ -203,3 +203,18 @@ def test_a_norm_within_the_state_is_refused(k):
     at = row[k] + (0 if k == 5 else 4)
     assert adam_call([adam_row(9 * FAKE, 10 * FAKE, 11 * FAKE, 12 * FAKE, step=13 * FAKE), row], norm_kind=2, max_norm=1.0,
                      norm=at, ws=16 * FAKE) == 5
+
+
+def test_the_host_library_goes_with_its_torch(monkeypatch):
+    """Another torch: `make` builds the host library anew, and one that was not built anew is refused."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__)))
+    version = os.path.join(os.path.dirname(torch.__file__), "version.py")
+    plan = ["make", "-n", "-C", root, "v2e2v_amd/libcista_torch.so"]
+    assert "cista_torch.cpp" in subprocess.run(plan + ["-W", version], capture_output=True, text=True, check=True).stdout
+    _lib.torch_lib()
+    monkeypatch.setattr(_lib, "_torch_lib", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0+rocm1.0")
+    with pytest.raises(_lib.CistaError, match="built for torch"):
+        optim.grad_norm([torch.ones(1)])

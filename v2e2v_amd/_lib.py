@@ -180,7 +180,14 @@ def torch_lib():
         lib()
         if not os.path.exists(TORCH_LIB_PATH):
             raise CistaError(f"libcista_torch.so not found at {TORCH_LIB_PATH}; build it first (`make`)")
-        t = ctypes.PyDLL(TORCH_LIB_PATH)
+        try:
+            t = ctypes.PyDLL(TORCH_LIB_PATH)
+            t.cista_torch_version.restype = ctypes.c_char_p
+            built = t.cista_torch_version().decode()
+        except (OSError, AttributeError) as e:
+            raise CistaError(f"failed to load {TORCH_LIB_PATH} (built for another torch?): {e}; build it again (`make`)") from e
+        if built != re.match(r"[\d.]*\d", torch.__version__).group():
+            raise CistaError(f"{TORCH_LIB_PATH} was built for torch {built}, this is {torch.__version__}; build it again (`make`)")
         obj, dbl = ctypes.py_object, ctypes.c_double
         for name, args in (("cista_torch_grad_norm", [obj, c_int]), ("cista_torch_clip_grads", [obj, c_int, dbl]),
                            ("cista_torch_adam_step", [obj, obj, c_int, dbl])):

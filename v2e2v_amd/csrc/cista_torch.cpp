@@ -11,6 +11,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <cmath>
 #include <vector>
@@ -169,6 +170,9 @@ float *moment(PyObject *slot, PyObject *key, const at::Tensor &p, int &device) {
 }  // namespace
 
 extern "C" {
+
+// the torch whose headers this was built with: another one's tensors may be laid out in another way
+const char *cista_torch_version() { return TORCH_VERSION; }
 
 // the norm of the list's tensors
 PyObject *cista_torch_grad_norm(PyObject *tensors, int norm_kind) {
