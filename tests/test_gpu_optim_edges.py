@@ -340,3 +340,69 @@ def test_a_norm_that_is_a_gradient_is_refused():
     with pytest.raises(_lib.CistaError, match="overlaps"):
         optim.clip_grads_with_norm_(params_of(grads), 1e-3, grads[1][7])
     assert all(torch.equal(a, b) for a, b in zip(grads, old))
+
+
+# --------------------------------------------------------------------------- past the cache's size
+GUARD = 3
+
+
+def flat_of(sizes, dtype, seed, scale, off, draw=torch.randn):
+    """Views end to end in one buffer that begins `off` elements in, and the buffer."""
+    flat = draw(sum(sizes) + off + GUARD, device=DEV, generator=gen(seed)).mul_(scale).to(dtype)
+    got, at = [], off
+    for n in sizes:
+        got.append(flat[at:at + n])
+        at += n
+    return got, flat
+
+
+def large_sizes(count):
+    """10.9 M elements in `count` tensors: a few large ones, odd ones, small ones and empty ones."""
+    sizes = [n % 97 for n in range(count - 5)] + [1025, 777_777, 1_500_001, 3_600_003]
+    return sizes + [10_900_000 - sum(sizes)]
+
+
+@pytest.mark.parametrize("order", [1, 2, math.inf])
+@pytest.mark.parametrize("count", [37, 64, 150])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_steps_with_clipping(dtype, count, order):
+    """More bytes than the last-level cache holds: one table and several, one group and two, every array of
+    tensors end to end at an odd place of its own, and nothing written beside them."""
+    sizes = large_sizes(count)
+    assert sum(sizes) * 28 > 256 << 20
+    half = dtype != torch.float32
+    w, wf = flat_of(sizes, dtype, 1, 0.1, 3)
+    g, gf = flat_of(sizes, dtype, 2, 0.3, 1)
+    m, mf = flat_of(sizes, torch.float32, 3, 0.1, 5)
+    v, vf = flat_of(sizes, torch.float32, 4, 0.05, 2, torch.rand)
+    master, af = flat_of(sizes, torch.float32, 5, 0.1, 7) if half else (w, wf)
+    ps = [torch.nn.Parameter(x) for x in w]
+    for p, x in zip(ps, g):
+        p.grad = x
+    hyper = dict(HYPER, weight_decay=0.05, decoupled=True)
+    kw = dict(lr=hyper["lr"], weight_decay=0.05, max_norm=0.2, norm_type=order)
+    opt = optim.AdamW(ps if count != 150 else [dict(params=ps[:80]), dict(params=ps[80:])], **kw)
+    steps = torch.full((len(ps),), 6.0, device=DEV)
+    for i, p in enumerate(ps):
+        opt.state[p] = dict(step=steps[i], exp_avg=m[i], exp_avg_sq=v[i], **({"master": master[i]} if half else {}))
+    norm = norm64(g, order)
+    before = snapshot(opt, ps, {})
+    kept = gf.clone()
+    arrays = [wf, mf, vf] + ([af] if half else [])
+    ends = [(x[:o].clone(), x[-GUARD:].clone()) for x, o in zip(arrays, (3, 5, 2, 7))]
+    opt.step()
+    near(opt.grad_norm, norm, order)
+    check_step(opt, ps, before, hyper, 7, min(1.0, 0.2 / (norm + 1e-6)))
+    assert torch.equal(gf, kept)
+    for x, o, (a, b) in zip(arrays, (3, 5, 2, 7), ends):
+        assert torch.equal(x[:o], a) and torch.equal(x[-GUARD:], b)
+
+
+@pytest.mark.parametrize("order", [1, 2, math.inf])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norms_of_more_than_the_cache_holds(dtype, order):
+    size = 2 if dtype != torch.float32 else 4
+    n = (280 << 20) // size
+    ts, _ = flat_of([5, n // 3, 1, n // 2, 999, n // 6], dtype, 8, 1e-3 if order == 1 else 1.0, 1)
+    assert sum(t.numel() for t in ts) * size > 256 << 20
+    near(optim.grad_norm(ts, order), norm64(ts, order), order)
