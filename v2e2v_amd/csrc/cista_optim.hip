@@ -19,7 +19,7 @@ namespace cista_optim {
 
 constexpr int THREADS = 256;
 constexpr int NORM_TENSORS = 192;        // 20 B each in the kernel argument
-constexpr int NORM_BLOCKS = 1024;        // partial sums of one launch: the blocks that run at once (92 VGPRs)
+constexpr int NORM_BLOCKS = 1024;        // partial sums of one launch: see norm_partials
 constexpr int NORM_UNROLL = 4;           // 16-byte loads in flight per thread
 constexpr int NORM_CHUNK = THREADS * 16 * NORM_UNROLL;                   // bytes
 constexpr int LINE = 128;                // bytes of a cache line
@@ -243,8 +243,9 @@ __device__ void norm_chunk(Running<KIND> (&acc)[NORM_UNROLL], const Chunk<T> &c)
 }
 
 // Bound by HBM reads (600 M bf16: 186 us, 6.5 TB/s), or for few elements by the latency of a launch and
-// its join.  A block steps through the chunks; 2048 blocks, half of which wait for a place, take 189 us
-// and leave twice as many values to join (22 M float32, norm and scale: 39 -> 42 us).
+// its join.  A block steps through the chunks; 2048 blocks take 189 us and leave twice as many values to
+// join (clip of 22 M float32 54.8 -> 55.4 us, Adam of 22 M with clipping 118.7 -> 119.5), but behind a copy
+// the clip of 150 M bf16 takes 283 us with them instead of 289.
 template <int KIND, bool STREAM, int N>
 __device__ void norm_partials(const NormTable<N> &t, double *partials, uint32_t blocks) {
     const Finder<N> find(t.first);
@@ -307,9 +308,10 @@ __device__ inline float norm_of(int kind, const double *partials, int n) {
 // Where a kernel takes its norm from: *given, or (given == nullptr) the partial values of the
 // launches before it.  Every block then joins them for itself, in the same order and so to the same
 // bits, and block 0 writes the norm down.  For few partial values and one consumer that is cheaper
-// than a launch that does it once (network of 1.4 M parameters, 343 values: 27.5 -> 21.6 us for the
-// step), but 22 M parameters with 2048 values take 124.6 us with the join of its own and 130 without,
-// 200 M bf16 in 5 launches 1435 and 1452 us: see JOIN_ALL.
+// than a launch that does it once (network of 1.4 M parameters, 358 values: 27.5 -> 21.6 us for the
+// step), but 22 M parameters with 1024 values take 118.7 us with the join of its own and 120.1 without
+// (clip: 54.8 and 55.8), 200 M bf16 in 5 launches (of up to 2048 values then) 1435 and 1452 us: see
+// JOIN_ALL.
 struct NormSource {
     const float *given;
     const double *partials;
@@ -432,12 +434,13 @@ __device__ void adam_chunk(T *p, const T *g, float *m, float *v, float *w, int64
 }
 
 // Seven streams over HBM, 28 bytes and some 40 operations an element: bound by HBM (268 M float32:
-// 1195 us, 6.3 TB/s, where a 4 GiB copy reaches 4.9), or by launches where it is small.  One block
+// 1201 us, 6.25 TB/s, where a 4 GiB copy reaches 4.9), or by launches where it is small.  One block
 // per chunk, dispatched in the order of the addresses: 2048 blocks that step through the chunks drift
 // apart and lose the DRAM's pages (1632 us against 1404, before the lines and STREAM).  Where all of it
 // fits the last-level cache STREAM costs (1.4 M parameters: 8.5 -> 9.5 us; 268 M: 1404 -> 1358), so
 // it goes by the bytes, and so does FIVE: with 5 blocks on a CU instead of 8 the blocks stay closer
-// together (1249 -> 1195 us, 6.3 TB/s; 3 blocks 1237; 1.4 M parameters: 9.0 -> 9.3 us).  The blocks of an
+// together (the step of 268 M with clipping 1422 -> 1363 us, 3 blocks 1379; of 200 M bf16 998 -> 981 and 1004;
+// of 22 M 120.8 -> 118.5 and 121.2; 1.4 M parameters: update 9.0 -> 9.3).  The blocks of an
 // XCD (block mod 8) take the chunks whose gradients its L2 has from the norm: 4 of them to a chunk of
 // the norm's.
 template <bool STREAM>
