@@ -12,7 +12,7 @@ OBJ  = build/cista_abi.o build/cista_voxel.o build/cista_ssim.o build/cista_v2e.
 # host library between Python's lists of tensors and the C ABI (links the installed torch)
 TLIB  = v2e2v_amd/libcista_torch.so
 PY    ?= python3
-TORCH := $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(u.find_spec('torch').origin))")
+TORCH := $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(u.find_spec('torch').origin))" 2>/dev/null)
 PYINC = $(shell $(PY) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
 
 all: $(LIB) $(TLIB)

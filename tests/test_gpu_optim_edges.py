@@ -85,6 +85,21 @@ def test_second_moment_of_a_small_beta2(dtype, b2):
         assert bool((off <= bound).all()), float((off / bound).max())
 
 
+@pytest.mark.parametrize("b2", [0.0, 0.3, 0.9])
+def test_an_overflowed_second_moment_stays_infinite(b2):
+    """Its weights stay where they are, and its neighbours go on."""
+    p = torch.nn.Parameter(torch.ones(4099, device=DEV))
+    opt = optim.Adam([p], lr=0.1, betas=(0.9, b2))
+    big = torch.zeros(4099, dtype=torch.bool, device=DEV)
+    big[[0, 1027, 4098]] = True
+    for scale in (1e21, 1.0):
+        p.grad = torch.where(big, scale, 1.0)
+        opt.step()
+    v = opt.state[p]["exp_avg_sq"]
+    assert bool(v[big].isinf().all()) and bool((p.detach()[big] == 1.0).all())
+    assert bool(((v[~big] - 1.0).abs() < 1.0).all()) and bool((p.detach()[~big] < 0.9).all())
+
+
 # ------------------------------------------------------------------------------------- one rounding
 def near_ties(dtype, seed):
     """A scale c (float32) and values g of the type for which the float32 product, rounded to the type, differs from

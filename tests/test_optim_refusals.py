@@ -195,6 +195,7 @@ def test_a_norm_within_the_tensors_is_refused(norm):
     t = table((FAKE, 16, 0), (FAKE * 8, 3, 0))
     assert L.cista_scale_grads(t, 2, 1.0, norm, None) == 5
     assert L.cista_clip_grads(t, 2, 2, 1.0, norm, FAKE * 16, 1 << 30, None) == 5
+    assert L.cista_scale_grads(table((norm + 2, 0, 1)), 1, 1.0, norm, None) != 5        # an empty one holds nothing
 
 
 @pytest.mark.parametrize("k", [0, 1, 2, 3, 4, 5])

@@ -380,10 +380,10 @@ __device__ inline float moment1(float m, float g, const AdamArgs &a) {
 
 // b2 v + (1 - b2) g^2, with b2 v as v - (1 - b2) v: b2 itself, rounded, would move the average of a long
 // run by 2^-24 / (1 - b2).  Below 1/2 it is the other way round (b2 = 1e-9: 1 - b2 is 1, and nothing
-// of v would be left).
+// of v would be left).  An average that has overflowed stays infinite, whatever b2 is.
 __device__ inline float moment2(float v, float g, const AdamArgs &a) {
-    const float kept = a.rate2 > 0.5f ? a.beta2 * v : v < __builtin_inff() ? fmaf(-a.rate2, v, v) : v;
-    return fmaf(a.rate2 * g, g, kept);
+    const float kept = a.rate2 > 0.5f ? a.beta2 * v : fmaf(-a.rate2, v, v);
+    return fmaf(a.rate2 * g, g, v < __builtin_inff() ? kept : v);
 }
 
 __device__ inline void adam_element(float &p, float g, float &m, float &v, const AdamArgs &a, const Rates &r, float c) {
@@ -519,7 +519,7 @@ Range range_of(const void *data, long long numel, long long type) {
 // is the float x within the tensor?  A norm is read, or written, by some workgroups while others write theirs
 bool holds(const float *x, const void *data, long long numel, long long type) {
     const Range r = range_of(data, numel, type);
-    return (uintptr_t)x < r.end && (uintptr_t)x + sizeof(float) > r.begin;
+    return numel && (uintptr_t)x < r.end && (uintptr_t)x + sizeof(float) > r.begin;
 }
 
 bool holds(const float *x, const cista_tensor *t, int n) {
