@@ -80,3 +80,23 @@ def test_gradients_cleared_by_a_hook_of_the_step(closure):
     before = [(p._version, p.detach().clone()) for p in params]
     opt.step(loss if closure else None)
     assert all(p.grad is None and p._version > v and not torch.equal(p.detach(), old) for p, (v, old) in zip(params, before))
+
+
+def test_gradients_cleared_by_a_global_hook():
+    """One that was registered before this package's runs before it."""
+    from torch.optim.optimizer import _global_optimizer_post_hooks as hooks
+    from torch.optim.optimizer import register_optimizer_step_post_hook
+    handle = register_optimizer_step_post_hook(lambda o, args, kwargs: o.zero_grad())
+    try:
+        hooks.move_to_end(handle.id, last=False)
+        params = with_grads(list(small().parameters()))
+        before = [p._version for p in params]
+        net = small()                                        # of other parameters: they were not stepped
+        torch.optim.Adam(params, lr=0.1, fused=True).step()
+        assert [p._version for p in params] == before        # their network is gone
+        params = with_grads(list(net.parameters()))
+        before = [p._version for p in params]
+        torch.optim.Adam(params, lr=0.1, fused=True).step()
+        assert all(p.grad is None and p._version > v for p, v in zip(params, before))
+    finally:
+        handle.remove()

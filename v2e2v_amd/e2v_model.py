@@ -29,30 +29,17 @@ import weakref
 
 import torch
 import torch.nn as nn
-from torch.optim.optimizer import register_optimizer_step_post_hook, register_optimizer_step_pre_hook
+from torch.optim.optimizer import _global_optimizer_post_hooks, register_optimizer_step_post_hook
 
 from . import _lib
 from .base_layers import ConvLayer, ConvLSTC, IstaBlock, RecurrentConvLayer, UpsampleConvLayer
 
 
 _networks = weakref.WeakSet()                 # every CistaLSTCNet there is
-_to_step = weakref.WeakKeyDictionary()        # optimizer: memory of the parameters of its running step
 
 
 def _memory(p):
     return p.untyped_storage()._cdata if p.layout == torch.strided else id(p)
-
-
-def _fused_memory(optimizer, every=False):
-    return {_memory(p) for g in optimizer.param_groups if g.get("fused") for p in g["params"] if every or p.grad is not None}
-
-
-def _before_step(optimizer, args, kwargs):
-    """Notes what a fused step is about to write: an optimizer's own post-hooks, which run before
-    _versions_after_fused_step, may clear the gradients.  A closure makes them within the step: all
-    parameters count then."""
-    every = any(a is not None for a in args[1:]) or any(a is not None for a in kwargs.values())
-    _to_step[optimizer] = _fused_memory(optimizer, every)
 
 
 def _versions_after_fused_step(optimizer, args, kwargs):
@@ -60,13 +47,16 @@ def _versions_after_fused_step(optimizer, args, kwargs):
     packed_params and _grad_conduit go by: a network trained with one kept its first packed
     weights.  This runs after every optimizer step and advances those of the networks' parameters in
     the memory that was stepped (they may be views of a flat one); other models' stay as they are."""
-    stepped = _to_step.pop(optimizer, set()) | _fused_memory(optimizer)
-    if stepped:
-        own = [p for net in list(_networks) if "_parameters" in net.__dict__ for p in net.parameters()]
-        torch.autograd.graph.increment_version([p for p in own if _memory(p) in stepped])
+    fused = [g for g in optimizer.param_groups if g.get("fused")]
+    if not fused:
+        return
+    # hooks that ran before this one may have cleared the gradients: then all parameters count
+    every = optimizer._optimizer_step_post_hooks or len(_global_optimizer_post_hooks) > 1
+    stepped = {_memory(p) for g in fused for p in g["params"] if every or p.grad is not None}
+    own = [p for net in list(_networks) if "_parameters" in net.__dict__ for p in net.parameters()]
+    torch.autograd.graph.increment_version([p for p in own if _memory(p) in stepped])
 
 
-register_optimizer_step_pre_hook(_before_step)
 register_optimizer_step_post_hook(_versions_after_fused_step)
 
 
